@@ -286,6 +286,23 @@ int npb_q_embedding(const int64_t* ids, int64_t T, const npb_q_weight* w, int64_
                     int64_t padding_idx, float embed_scale, void* out, int out_dtype,
                     npb_stream_t stream);
 
+/* ---- reading logits ------------------------------------------------------------------ */
+
+#define NPB_LOGPROBS_MAX_TOP 32
+
+/* Log probabilities from logits [R, V] (row stride ld elements, ld >= V; NPB_BF16 / NPB_F16 /
+ * NPB_F32, any alignment of the rows down to the element's), fp32 sums, natural logarithm:
+ *   logprob[r]  = l[r, targets[r]] - lse_r, lse_r = ln sum_v e^l[r, v]; 0 for a target outside [0, V)
+ *   entropy[r]  = -sum_v p_v ln p_v
+ *   top_logprobs[r, :], top_ids[r, :] (int64): the top_n (0..NPB_LOGPROBS_MAX_TOP, <= V) largest
+ *   logits as log probabilities, equal logits by ascending index; may be NULL for top_n 0.
+ * -inf logits have probability 0.  A row of nothing but -inf: log probabilities -inf, entropy 0.  A
+ * row with NaN or +inf: NaN, top_ids by value with NaN last.  One kernel, each logit read from
+ * HBM once.  R < 2^27, V < 2^30.  No reference counterpart. */
+int npb_token_logprobs(const void* logits, int64_t ld, int64_t R, int64_t V, int dtype,
+                       const int64_t* targets, int top_n, float* logprob, float* entropy,
+                       float* top_logprobs, int64_t* top_ids, npb_stream_t stream);
+
 /*
  * Multi-GPU (new; the reference has no distributed code): all-gather of out-feature shards by
  * pushing.  This rank's src[M, n_local] (elem_bytes per element) is stored into columns

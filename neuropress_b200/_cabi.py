@@ -19,6 +19,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libneuropress_b200.so"
 
 NPB_F16, NPB_BF16, NPB_F32 = 0, 1, 2
 GEMV_MAX_ROWS = 8
+LOGPROBS_MAX_TOP = 32
 STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 
 _DTYPE_CODE = {torch.float16: NPB_F16, torch.bfloat16: NPB_BF16, torch.float32: NPB_F32}
@@ -50,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "npb_rms_norm",
     "npb_vq_embedding",
     "npb_q_embedding",
+    "npb_token_logprobs",
     "npb_gemm_device_status",
     "npb_set_wait_limit_ns",
     "npb_get_wait_limit_ns",
@@ -174,6 +176,8 @@ def load_library() -> ctypes.CDLL:
                                      c_void_p, ctypes.c_float, c_void_p, c_int, c_void_p]
     lib.npb_q_embedding.argtypes = [c_void_p, c_int64, q_p, c_int64, c_int64, c_int64, ctypes.c_float, c_void_p,
                                     c_int, c_void_p]
+    lib.npb_token_logprobs.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_void_p]
     lib.npb_gemm_device_status.argtypes = [POINTER(c_int)]
     lib.npb_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     lib.npb_get_wait_limit_ns.argtypes = []

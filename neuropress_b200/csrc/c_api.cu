@@ -44,6 +44,8 @@ int vq_embedding(const int64_t*, int64_t, const uint16_t*, int64_t, int64_t, con
                  float, void*, int, cudaStream_t);
 int q_embedding(const int64_t*, int64_t, const npb_q_weight*, int64_t, int64_t, int64_t, float, void*, int,
                 cudaStream_t);
+int token_logprobs(const void*, int64_t, int64_t, int64_t, int, const int64_t*, int, float*, float*, float*, int64_t*,
+                   cudaStream_t);
 int gemm_gather(const void*, const void*, const float*, int64_t, int64_t, int64_t, int, const GatherSink&,
                 cudaStream_t);
 int vq_gemv_gather(const npb_vq_weight*, const void*, int, int64_t, int64_t, int64_t, const float*,
@@ -324,6 +326,13 @@ int npb_q_embedding(const int64_t* ids, int64_t T, const npb_q_weight* w, int64_
                     int64_t padding_idx, float embed_scale, void* out, int out_dtype, npb_stream_t stream) {
   return npb::q_embedding(ids, T, w, V, D, padding_idx, embed_scale, out, out_dtype,
                           static_cast<cudaStream_t>(stream));
+}
+
+int npb_token_logprobs(const void* logits, int64_t ld, int64_t R, int64_t V, int dtype, const int64_t* targets,
+                       int top_n, float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids,
+                       npb_stream_t stream) {
+  return npb::token_logprobs(logits, ld, R, V, dtype, targets, top_n, logprob, entropy, top_logprobs, top_ids,
+                             static_cast<cudaStream_t>(stream));
 }
 
 int npb_gemm_device_status(int* host_out) { return npb::gemm_device_status(host_out); }

@@ -635,3 +635,40 @@ def q_embedding(input_ids: torch.Tensor, u8_blob: torch.Tensor, scale: torch.Ten
                      _cabi.dtype_code(dt), _cabi.stream_ptr())
     _cabi.check(rc, "q_embedding")
     return out.reshape(*input_ids.shape, d)
+
+
+# ---------------------------------------------------------------------------
+# Reading logits
+# ---------------------------------------------------------------------------
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Log probabilities of given tokens, entropy and the ``top_n`` most likely tokens, from
+    ``logits`` ``[R, V]`` (bf16, fp16 or fp32; rows may be strided, e.g. ``padded[:, :V]``) and
+    ``targets`` int64 ``[R]``.  Returns ``(logprob [R], entropy [R], top_logprobs [R, top_n],
+    top_ids [R, top_n])``: fp32, natural logarithm, ids int64, equal logits by ascending id.  A target
+    outside ``[0, V)`` (an ignore index) yields log probability 0.  ``-inf`` logits are masked
+    tokens; a fully masked row gives ``-inf`` and entropy 0, a row with NaN or ``+inf`` gives NaN.
+    No reference counterpart."""
+    if logits.dim() != 2 or targets.dim() != 1 or targets.shape[0] != logits.shape[0]:
+        raise RuntimeError("token_logprobs: expected logits [R, V] and targets [R].")
+    if targets.dtype != torch.int64:
+        raise RuntimeError("token_logprobs: targets must be int64.")
+    r, v = logits.shape
+    if v == 0 or not 0 <= top_n <= min(v, _cabi.LOGPROBS_MAX_TOP):
+        raise RuntimeError(f"token_logprobs: top_n must lie in [0, min(V, {_cabi.LOGPROBS_MAX_TOP})], V > 0.")
+    if v > 1 and logits.stride(1) != 1 or r > 1 and logits.stride(0) < v:
+        raise RuntimeError("token_logprobs: the rows of logits must be contiguous and must not overlap.")
+    _cabi.require_cuda("token_logprobs", targets, logits[:1])   # rows may be strided
+    lib = _cabi.load_library()
+    code = _cabi.dtype_code(logits.dtype)
+    logprob, entropy = torch.empty((2, r), dtype=torch.float32, device=logits.device)
+    top = torch.empty((r, top_n), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((r, top_n), dtype=torch.int64, device=logits.device)
+    with torch.cuda.device(logits.device):
+        rc = _launch("npb_token_logprobs", lib.npb_token_logprobs, logits.data_ptr(), logits.stride(0) if r > 1 else v,
+                     r, v, code, targets.data_ptr(), int(top_n), logprob.data_ptr(), entropy.data_ptr(),
+                     top.data_ptr(), ids.data_ptr(), _cabi.stream_ptr())
+    _cabi.check(rc, "token_logprobs")
+    return logprob, entropy, top, ids
