@@ -286,6 +286,30 @@ int npb_q_embedding(const int64_t* ids, int64_t T, const npb_q_weight* w, int64_
                     int64_t padding_idx, float embed_scale, void* out, int out_dtype,
                     npb_stream_t stream);
 
+/* ---- mixture of experts ---------------------------------------------------------------- */
+
+#define NPB_MOE_MAX_TOKENS 32
+#define NPB_MOE_MAX_EXPERTS 512
+#define NPB_MOE_MAX_TOP_K 16
+
+/* A mixture-of-experts layer for up to NPB_MOE_MAX_TOKENS tokens over 4-bit group-affine experts:
+ *   p = softmax(logits[t, :E]);  S = the top_k largest logits (equal logits: lowest expert)
+ *   w_e = p_e, or p_e / sum_S p if renormalize
+ *   y[t] = T( sum_{e in S} w_e * D_e ( silu(G_e x[t]) * (U_e x[t]) ) )          fp32 arithmetic
+ * x, y [T, H] in dtype (NPB_BF16 / NPB_F16), logits [T, E] in logits_dtype (also NPB_F32).  gate / up
+ * are the experts' [I, H] weights stacked to [E * I, H], down the [H, I] weights stacked to
+ * [E * H, I]; nbits 4, group_size a multiple of 32, codes 16-byte aligned, gate and up both with or
+ * both without zero points.  H, I multiples of 32.  Experts with logit -inf are not used, a token
+ * whose logits are all -inf yields zeros, one with NaN or +inf yields NaN.  workspace: 16-byte
+ * aligned, npb_q_moe_workspace_bytes, not shared by calls that may run at the same time; its
+ * content need not be kept or cleared.  Two kernels; the same bits for the same inputs every time.  No
+ * reference counterpart: the reference runs every expert's linears by themselves. */
+int64_t npb_q_moe_workspace_bytes(int64_t T, int top_k, int64_t I); /* 0: sizes out of range */
+int npb_q_moe(const void* x, int dtype, const void* logits, int logits_dtype, int64_t T, int64_t E,
+              int64_t H, int64_t I, const npb_q_weight* gate, const npb_q_weight* up,
+              const npb_q_weight* down, int top_k, int renormalize, void* workspace,
+              int64_t workspace_bytes, void* y, npb_stream_t stream);
+
 /* ---- reading logits ------------------------------------------------------------------ */
 
 #define NPB_LOGPROBS_MAX_TOP 32

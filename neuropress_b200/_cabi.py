@@ -20,6 +20,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libneuropress_b200.so"
 NPB_F16, NPB_BF16, NPB_F32 = 0, 1, 2
 GEMV_MAX_ROWS = 8
 LOGPROBS_MAX_TOP = 32
+MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 32, 512, 16
 STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 
 _DTYPE_CODE = {torch.float16: NPB_F16, torch.bfloat16: NPB_BF16, torch.float32: NPB_F32}
@@ -51,6 +52,8 @@ EXPORTED_SYMBOLS = (
     "npb_rms_norm",
     "npb_vq_embedding",
     "npb_q_embedding",
+    "npb_q_moe_workspace_bytes",
+    "npb_q_moe",
     "npb_token_logprobs",
     "npb_gemm_device_status",
     "npb_set_wait_limit_ns",
@@ -176,6 +179,9 @@ def load_library() -> ctypes.CDLL:
                                      c_void_p, ctypes.c_float, c_void_p, c_int, c_void_p]
     lib.npb_q_embedding.argtypes = [c_void_p, c_int64, q_p, c_int64, c_int64, c_int64, ctypes.c_float, c_void_p,
                                     c_int, c_void_p]
+    lib.npb_q_moe_workspace_bytes.argtypes = [c_int64, c_int, c_int64]
+    lib.npb_q_moe.argtypes = [c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, q_p, q_p, q_p, c_int,
+                              c_int, c_void_p, c_int64, c_void_p, c_void_p]
     lib.npb_token_logprobs.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p]
     lib.npb_gemm_device_status.argtypes = [POINTER(c_int)]
@@ -186,6 +192,7 @@ def load_library() -> ctypes.CDLL:
     for name in EXPORTED_SYMBOLS[3:]:
         getattr(lib, name).restype = c_int
     lib.npb_get_wait_limit_ns.restype = ctypes.c_uint64
+    lib.npb_q_moe_workspace_bytes.restype = c_int64
     _lib = lib
     return lib
 

@@ -44,6 +44,9 @@ int vq_embedding(const int64_t*, int64_t, const uint16_t*, int64_t, int64_t, con
                  float, void*, int, cudaStream_t);
 int q_embedding(const int64_t*, int64_t, const npb_q_weight*, int64_t, int64_t, int64_t, float, void*, int,
                 cudaStream_t);
+int64_t q_moe_workspace_bytes(int64_t, int, int64_t);
+int q_moe(const void*, int, const void*, int, int64_t, int64_t, int64_t, int64_t, const npb_q_weight*,
+          const npb_q_weight*, const npb_q_weight*, int, int, void*, int64_t, void*, cudaStream_t);
 int token_logprobs(const void*, int64_t, int64_t, int64_t, int, const int64_t*, int, float*, float*, float*, int64_t*,
                    cudaStream_t);
 int gemm_gather(const void*, const void*, const float*, int64_t, int64_t, int64_t, int, const GatherSink&,
@@ -326,6 +329,15 @@ int npb_q_embedding(const int64_t* ids, int64_t T, const npb_q_weight* w, int64_
                     int64_t padding_idx, float embed_scale, void* out, int out_dtype, npb_stream_t stream) {
   return npb::q_embedding(ids, T, w, V, D, padding_idx, embed_scale, out, out_dtype,
                           static_cast<cudaStream_t>(stream));
+}
+
+int64_t npb_q_moe_workspace_bytes(int64_t T, int top_k, int64_t I) { return npb::q_moe_workspace_bytes(T, top_k, I); }
+
+int npb_q_moe(const void* x, int dtype, const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t H,
+              int64_t I, const npb_q_weight* gate, const npb_q_weight* up, const npb_q_weight* down, int top_k,
+              int renormalize, void* workspace, int64_t workspace_bytes, void* y, npb_stream_t stream) {
+  return npb::q_moe(x, dtype, logits, logits_dtype, T, E, H, I, gate, up, down, top_k, renormalize, workspace,
+                    workspace_bytes, y, static_cast<cudaStream_t>(stream));
 }
 
 int npb_token_logprobs(const void* logits, int64_t ld, int64_t R, int64_t V, int dtype, const int64_t* targets,

@@ -17,6 +17,7 @@
 // bound ties with most of the row) find the exact n-th value by bisection over the ordered bits of the
 // values and take the ties in index order.
 #include "common.cuh"
+#include "order_key.cuh"
 #include "tcgen05.cuh"
 
 namespace npb {
@@ -41,17 +42,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Order-preserving bits of a float: larger value, larger key; -0 counts as +0, NaN sorts last (1),
-// 0 is no element at all.
-__device__ __forceinline__ uint32_t order_key(float f) {
-  if (f != f) return 1u;
-  const uint32_t b = __float_as_uint(f + 0.f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  if (k <= 1u) return __int_as_float(0x7fc00000);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
 // (value, index): larger value first, equal values by ascending index.
 __device__ __forceinline__ uint64_t full_key(uint32_t k, int index) {
   return ((uint64_t)k << 32) | (uint32_t)~index;

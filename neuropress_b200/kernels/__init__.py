@@ -555,6 +555,70 @@ def q_linear(x: torch.Tensor, w_pack: torch.Tensor, scale: torch.Tensor, nbits: 
 
 
 # ---------------------------------------------------------------------------
+# Mixture of experts (group-affine experts)
+# ---------------------------------------------------------------------------
+
+
+def _moe_weight(name: str, weight: tuple, e: int, rows: int, k: int, group_size: int):
+    codes, scale, zero_point = weight
+    if tuple(codes.shape) != (e, rows, k // 2):
+        raise RuntimeError(f"q_moe: the codes of {name} must be [{e}, {rows}, {k // 2}], got {list(codes.shape)}.")
+    n_groups = e * rows * (k // group_size)
+    if scale.numel() != n_groups or (zero_point is not None and zero_point.numel() != n_groups):
+        raise RuntimeError(f"q_moe: scale / zero_point of {name} must have {n_groups} elements.")
+    return _cabi.q_struct(codes, scale, zero_point, 4, group_size)
+
+
+def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, down: tuple, top_k: int,
+          group_size: int, renormalize: bool = True) -> torch.Tensor:
+    """A mixture-of-experts layer for a few tokens over 4-bit group-affine experts, in two kernels:
+    softmax of ``router_logits`` ``[T, E]`` (fp32, bf16 or fp16), the ``top_k`` largest (equal logits:
+    lowest expert; weights renormalised to sum 1 if ``renormalize``), and
+    ``y[t] = sum_e w_e * down_e(silu(gate_e(x[t])) * up_e(x[t]))`` in fp32.  ``x`` is ``[T, H]`` bf16 or
+    fp16; ``gate``, ``up`` and ``down`` are ``(codes, scale, zero_point or None)`` with codes
+    ``[E, I, H/2]``, ``[E, I, H/2]``, ``[E, H, I/2]`` in the layout of :func:`q_linear`, scale / zero_point
+    one fp16 per group of ``group_size`` (a multiple of 32).  More than 32 tokens run 32 at a time.
+    An expert whose logit is ``-inf`` is not used; a token with no expert left yields zeros, one with NaN
+    or ``+inf`` logits yields NaN.  No reference counterpart (the reference runs each expert's
+    linears)."""
+    if x.dim() != 2 or router_logits.dim() != 2 or router_logits.shape[0] != x.shape[0]:
+        raise RuntimeError("q_moe: expected x [T, H] and router_logits [T, E].")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("q_moe: x must be float16 or bfloat16.")
+    t, h = x.shape
+    e = router_logits.shape[1]
+    if gate[0].dim() != 3:
+        raise RuntimeError("q_moe: codes must be 3-D, one matrix per expert.")
+    i = gate[0].shape[1]
+    if group_size <= 0 or group_size % 32 or h == 0 or i == 0 or h % group_size or i % group_size:
+        raise RuntimeError("q_moe: group_size must be a multiple of 32 that divides H and I.")
+    if not 1 <= top_k <= min(e, _cabi.MOE_MAX_TOP_K) or e > _cabi.MOE_MAX_EXPERTS:
+        raise RuntimeError(f"q_moe: top_k must lie in [1, min(E, {_cabi.MOE_MAX_TOP_K})], E in [1, "
+                           f"{_cabi.MOE_MAX_EXPERTS}].")
+    if (gate[2] is None) != (up[2] is None):
+        raise RuntimeError("q_moe: gate and up must both have zero points or both have none.")
+    structs = (_moe_weight("gate", gate, e, i, h, group_size), _moe_weight("up", up, e, i, h, group_size),
+               _moe_weight("down", down, e, h, i, group_size))
+    _cabi.require_cuda("q_moe", x, router_logits, *gate, *up, *down)
+    lib = _cabi.load_library()
+    code, logit_code = _cabi.dtype_code(x.dtype), _cabi.dtype_code(router_logits.dtype)
+    y = torch.empty_like(x)
+    if t == 0:
+        return y
+    n = min(t, _cabi.MOE_MAX_TOKENS)
+    size = lib.npb_q_moe_workspace_bytes(n, top_k, i)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    x_step, l_step = h * x.element_size(), e * router_logits.element_size()
+    with torch.cuda.device(x.device):
+        for t0 in range(0, t, n):
+            rc = _launch("npb_q_moe", lib.npb_q_moe, x.data_ptr() + t0 * x_step, code,
+                         router_logits.data_ptr() + t0 * l_step, logit_code, min(n, t - t0), e, h, i, *structs, top_k,
+                         int(renormalize), workspace.data_ptr(), size, y.data_ptr() + t0 * x_step, _cabi.stream_ptr())
+            _cabi.check(rc, "q_moe")
+    return y
+
+
+# ---------------------------------------------------------------------------
 # RMSNorm
 # ---------------------------------------------------------------------------
 
