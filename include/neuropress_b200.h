@@ -40,6 +40,15 @@ typedef enum {
 
 typedef enum { NPB_F16 = 0, NPB_BF16 = 1, NPB_F32 = 2 } npb_dtype;
 
+/* silu(v) = v / (1 + e^-v), gelu(v) = v * Phi(v), NPB_ACT_GELU_TANH its tanh approximation */
+typedef enum {
+  NPB_ACT_NONE = 0,
+  NPB_ACT_RELU = 1,
+  NPB_ACT_SILU = 2,
+  NPB_ACT_GELU = 3,
+  NPB_ACT_GELU_TANH = 4
+} npb_activation;
+
 /* Largest row count the fused GEMV kernels accept (the decode band is 1-2 rows by
  * default; up to this many rows are supported for tuning the band edge). */
 #define NPB_GEMV_MAX_ROWS 8
@@ -164,6 +173,14 @@ int npb_q_gemv(const npb_q_weight* w, const void* x, int x_dtype, int64_t M, int
  * pointers are required (TMA). */
 int npb_gemm(const void* x, const void* w, const float* bias, void* y, int64_t M, int64_t N,
              int64_t K, int dtype, npb_stream_t stream);
+
+/* y[M, N] = dtype( act(x[M, K] . w[N, K]^T + bias) + residual ): npb_gemm with an activation
+ * (npb_activation) and a residual [M, N] of dtype (or NULL) in its epilogue, everything before the
+ * last rounding in fp32.  Same operands and requirements as npb_gemm; residual may be y itself, but
+ * y must not overlap x, w or a shifted residual.  No reference counterpart (the reference runs
+ * cuBLAS and elementwise kernels). */
+int npb_gemm_epilogue(const void* x, const void* w, const float* bias, int activation, const void* residual,
+                      void* y, int64_t M, int64_t N, int64_t K, int dtype, npb_stream_t stream);
 
 /* Tile-decode GEMM: B tiles are decoded from the index stream straight into the swizzled
  * shared-memory stage, never written to HBM.  Replaces vq_gemm_triton

@@ -20,6 +20,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libneuropress_b200.so"
 NPB_F16, NPB_BF16, NPB_F32 = 0, 1, 2
 GEMV_MAX_ROWS = 8
 LOGPROBS_MAX_TOP = 32
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # npb_activation
 MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 32, 512, 16
 STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 
@@ -37,6 +38,7 @@ EXPORTED_SYMBOLS = (
     "npb_q_gemv",
     "npb_vq_gemv_grouped",
     "npb_gemm",
+    "npb_gemm_epilogue",
     "npb_vq_gemm_fused",
     "npb_vq_gemm_fused_cb",
     "npb_vq_codebook_cast",
@@ -166,6 +168,8 @@ def load_library() -> ctypes.CDLL:
     lib.npb_q_gemm_fused.argtypes = [q_p, *gemv_tail]
     lib.npb_gemm.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                              c_int, c_void_p]
+    lib.npb_gemm_epilogue.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64,
+                                      c_int64, c_int, c_void_p]
     lib.npb_allgather_push.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int,
                                        c_int, ctypes.c_uint32, c_void_p]
     sink_p = POINTER(GatherSinkStruct)

@@ -44,6 +44,8 @@ int vq_embedding(const int64_t*, int64_t, const uint16_t*, int64_t, int64_t, con
                  float, void*, int, cudaStream_t);
 int q_embedding(const int64_t*, int64_t, const npb_q_weight*, int64_t, int64_t, int64_t, float, void*, int,
                 cudaStream_t);
+int gemm_epilogue(const void*, const void*, const float*, int, const void*, void*, int64_t, int64_t, int64_t, int,
+                  cudaStream_t);
 int64_t q_moe_workspace_bytes(int64_t, int, int64_t);
 int q_moe(const void*, int, const void*, int, int64_t, int64_t, int64_t, int64_t, const npb_q_weight*,
           const npb_q_weight*, const npb_q_weight*, int, int, void*, int64_t, void*, cudaStream_t);
@@ -227,6 +229,11 @@ int npb_q_gemv(const npb_q_weight* w, const void* x, int x_dtype, int64_t M, int
 int npb_gemm(const void* x, const void* w, const float* bias, void* y, int64_t M, int64_t N,
              int64_t K, int dtype, npb_stream_t stream) {
   return npb::gemm(x, w, bias, y, M, N, K, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int npb_gemm_epilogue(const void* x, const void* w, const float* bias, int activation, const void* residual, void* y,
+                      int64_t M, int64_t N, int64_t K, int dtype, npb_stream_t stream) {
+  return npb::gemm_epilogue(x, w, bias, activation, residual, y, M, N, K, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int npb_vq_gemm_fused(const npb_vq_weight* w, const void* x, int x_dtype, int64_t M,

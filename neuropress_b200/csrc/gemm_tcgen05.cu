@@ -25,6 +25,7 @@
 #include <cstdlib>
 #include <type_traits>
 
+#include "activation.cuh"
 #include "common.cuh"
 #include "gather_sink.cuh"
 #include "q4_math.cuh"
@@ -64,6 +65,8 @@ struct GemmParams {
   FusedQ4 q4;
   GatherSink sink;  // peer_out != null: y goes to every rank's buffer, then the handshake
   uint64_t wait_ns;  // limit of every mbarrier wait (npb_set_wait_limit_ns; 2 s by default)
+  int act;               // EPI instantiations: npb_activation, applied after the bias,
+  const void* residual;  // and [M, N] of T (or null) added after it
 };
 
 template <int BN, int MT>
@@ -176,11 +179,13 @@ __device__ __forceinline__ void q4_emit(const Q4Item<RPL>& it, int n0, int N, ui
 // ---- the kernel ------------------------------------------------------------------------------
 // GATHER: the epilogue carries the fused all-gather (dense mode only); a separate instantiation
 // so that the plain kernels do not pay for its registers.
+// EPI: the epilogue applies an activation and adds a residual (npb_gemm_epilogue).  The four epilogue warps
+// work under the next tile's MMAs: 256 values a lane and tile against >= 8 K cycles of MMA from K = 2048 on.
 // CG = 2 (dense mode, MT = 1): two CTAs of a cluster share one 256 x BN tile -- each loads its own
 // 128 rows of x and its own BN/2 rows of W, the even CTA issues tcgen05.mma.cta_group::2 for both,
 // each CTA's TMEM gets the accumulator rows of its own x rows.  Half the W bytes per stage and CTA
 // means a deeper ring (7 stages instead of 4 at BN = 256) for the same shared memory.
-template <typename T, int BN, int MT, int BMODE, int BITS, bool GATHER, int CG = 1>
+template <typename T, int BN, int MT, int BMODE, int BITS, bool GATHER, int CG = 1, bool EPI = false>
 __global__ void __launch_bounds__(BMODE == B_TMA ? 192 : 192 + 32 * kQ4DecodeWarps, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
             const GemmParams p, const int stages) {
@@ -405,15 +410,26 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             const int64_t off = (int64_t)m * ld + col0 + n0;
             // 16-byte stores only where the destination address itself is 16-byte aligned (an
             // output that is a view at an odd offset takes the element-wise path)
-            const bool full = (n0 + 32 <= p.N) && ((reinterpret_cast<uintptr_t>(y + off) & 15u) == 0);
+            bool full = (n0 + 32 <= p.N) && ((reinterpret_cast<uintptr_t>(y + off) & 15u) == 0);
+            const T* res = EPI ? static_cast<const T*>(p.residual) : nullptr;
+            if (EPI && res) {
+              res += off;
+              full = full && (reinterpret_cast<uintptr_t>(res) & 15u) == 0;
+            }
             if (full) {
               struct alignas(16) Out { T e[8]; } o[4];
+              if (EPI && res) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[q] = reinterpret_cast<const Out*>(res)[q];
+              }
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                   float f = __uint_as_float(v[q * 8 + e]);
                   if (p.bias) f += __ldg(p.bias + n0 + q * 8 + e);
+                  if (EPI) f = activate(f, p.act);
+                  if (EPI && res) f += to_f32(o[q].e[e]);
                   o[q].e[e] = from_f32<T>(f);
                 }
               }
@@ -427,6 +443,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                 if (n0 + e < p.N) {
                   float f = __uint_as_float(v[e]);
                   if (p.bias) f += __ldg(p.bias + n0 + e);
+                  if (EPI) f = activate(f, p.act);
+                  if (EPI && res) f += to_f32(res[e]);
                   dst[e] = from_f32<T>(f);
                 }
               }
@@ -606,10 +624,10 @@ int pick_group_m(int tiles_m, int tiles_n, int tile_rows, int bn, int K, int cta
   return best_g;
 }
 
-template <typename T, int BN, int MT, int BMODE, int BITS, bool GATHER = false, int CG = 1>
+template <typename T, int BN, int MT, int BMODE, int BITS, bool GATHER = false, int CG = 1, bool EPI = false>
 int launch_gemm(const void* x, const void* w_dense, GemmParams p, cudaStream_t st) {
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  auto kern = gemm_kernel<T, BN, MT, BMODE, BITS, GATHER, CG>;
+  auto kern = gemm_kernel<T, BN, MT, BMODE, BITS, GATHER, CG, EPI>;
   using Layout = SmemLayout<BN / CG, MT>;  // a CTA of a pair holds half of the W tile
   const int cap = max_dynamic_smem();
   int stages = Layout::stages(cap);
@@ -714,23 +732,23 @@ bool use_pairs(int64_t M, int64_t N) {
   return (rows2 / (2 * BM)) * ((N + 255) / 256) >= sm_count() / 2;
 }
 
-template <typename T, bool GATHER>
+template <typename T, bool GATHER, bool EPI = false>
 int gemm_dense(const void* x, const void* w, GemmParams p, cudaStream_t st) {
   if (use_pairs(p.M, p.N)) {
     switch (pick_bn(p.M, p.N, 2)) {
-      case 256: return launch_gemm<T, 256, 1, B_TMA, 0, GATHER, 2>(x, w, p, st);
-      case 224: return launch_gemm<T, 224, 1, B_TMA, 0, GATHER, 2>(x, w, p, st);
-      case 192: return launch_gemm<T, 192, 1, B_TMA, 0, GATHER, 2>(x, w, p, st);
-      case 128: return launch_gemm<T, 128, 1, B_TMA, 0, GATHER, 2>(x, w, p, st);
-      default: return launch_gemm<T, 64, 1, B_TMA, 0, GATHER, 2>(x, w, p, st);
+      case 256: return launch_gemm<T, 256, 1, B_TMA, 0, GATHER, 2, EPI>(x, w, p, st);
+      case 224: return launch_gemm<T, 224, 1, B_TMA, 0, GATHER, 2, EPI>(x, w, p, st);
+      case 192: return launch_gemm<T, 192, 1, B_TMA, 0, GATHER, 2, EPI>(x, w, p, st);
+      case 128: return launch_gemm<T, 128, 1, B_TMA, 0, GATHER, 2, EPI>(x, w, p, st);
+      default: return launch_gemm<T, 64, 1, B_TMA, 0, GATHER, 2, EPI>(x, w, p, st);
     }
   }
   switch (pick_bn(p.M, p.N, 1)) {
-    case 256: return launch_gemm<T, 256, 1, B_TMA, 0, GATHER>(x, w, p, st);
-    case 224: return launch_gemm<T, 224, 1, B_TMA, 0, GATHER>(x, w, p, st);
-    case 192: return launch_gemm<T, 192, 1, B_TMA, 0, GATHER>(x, w, p, st);
-    case 128: return launch_gemm<T, 128, 1, B_TMA, 0, GATHER>(x, w, p, st);
-    default: return launch_gemm<T, 64, 1, B_TMA, 0, GATHER>(x, w, p, st);
+    case 256: return launch_gemm<T, 256, 1, B_TMA, 0, GATHER, 1, EPI>(x, w, p, st);
+    case 224: return launch_gemm<T, 224, 1, B_TMA, 0, GATHER, 1, EPI>(x, w, p, st);
+    case 192: return launch_gemm<T, 192, 1, B_TMA, 0, GATHER, 1, EPI>(x, w, p, st);
+    case 128: return launch_gemm<T, 128, 1, B_TMA, 0, GATHER, 1, EPI>(x, w, p, st);
+    default: return launch_gemm<T, 64, 1, B_TMA, 0, GATHER, 1, EPI>(x, w, p, st);
   }
 }
 
@@ -790,6 +808,25 @@ int gemm_impl(const void* x, const void* w, const float* bias, void* y, int64_t 
 int gemm(const void* x, const void* w, const float* bias, void* y, int64_t M, int64_t N, int64_t K,
          int dtype, cudaStream_t st) {
   return gemm_impl(x, w, bias, y, M, N, K, dtype, nullptr, st);
+}
+
+// y = T(act(x W^T + bias) + residual): the dense GEMM with the rest of a decoder block's step in its epilogue.
+int gemm_epilogue(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, int64_t M,
+                  int64_t N, int64_t K, int dtype, cudaStream_t st) {
+  if (act < NPB_ACT_NONE || act > NPB_ACT_GELU_TANH) return NPB_ERR_INVALID_ARG;
+  if (int rc = check_gemm_common(x, y, M, N, K, dtype)) return rc;
+  if (M == 0 || N == 0) return NPB_OK;
+  if (w == nullptr) return NPB_ERR_INVALID_ARG;
+  if (!aligned_to(w, 16) || !aligned_to(y, 2) || !aligned_to(residual, 2) || !aligned_to(bias, 4))
+    return NPB_ERR_ALIGNMENT;
+  GemmParams p{};
+  p.bias = bias;
+  p.y = y;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K;
+  p.act = act;
+  p.residual = residual;
+  return dtype == NPB_BF16 ? gemm_dense<__nv_bfloat16, false, true>(x, w, p, st)
+                           : gemm_dense<__half, false, true>(x, w, p, st);
 }
 
 // Dense GEMM whose epilogue stores this rank's [M, N] result into columns [col0, col0 + N) of

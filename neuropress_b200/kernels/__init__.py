@@ -377,14 +377,19 @@ def vq_lut_gather(lut: torch.Tensor, packed_indices: torch.Tensor, bits: int, ou
 
 
 def vq_dequant_gemm(x: torch.Tensor, packed_indices: torch.Tensor, centroids: torch.Tensor,
-                    bits: int, out_features: int | None = None, bias: torch.Tensor | None = None,
+                    bits: int, out_features: int | None = None, bias: torch.Tensor | None = None, *,
+                    activation: str | None = None, residual: torch.Tensor | None = None,
                     **ext) -> torch.Tensor:
     """One-pass decode to a temporary ``[N, K]`` weight in ``x.dtype``, then the dense
-    tensor-core GEMM (reference: ``_forward_dequant_gemm``, np_vq_linear.py:1127-1148)."""
+    tensor-core GEMM (reference: ``_forward_dequant_gemm``, np_vq_linear.py:1127-1148).
+    ``activation`` and ``residual`` (not in the reference) go into the GEMM's epilogue, see
+    :func:`gemm_epilogue`."""
     k = x.shape[1]
     n = out_features if out_features is not None else _infer_n(packed_indices, bits, k,
                                                                 centroids.shape[-1])
     w = vq_dequant(packed_indices, centroids, bits, n, k, x.dtype, **ext)
+    if activation is not None or residual is not None:
+        return gemm_epilogue(x, w, bias, activation, residual)
     return gemm(x, w, bias)
 
 
@@ -445,6 +450,35 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, gat
         rc = _launch("npb_gemm", lib.npb_gemm, x.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(),
                           y.data_ptr(), m, n, k, _cabi.dtype_code(x.dtype), _cabi.stream_ptr())
     _cabi.check(rc, "gemm")
+    return y
+
+
+def gemm_epilogue(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                  residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x[M,K] @ w[N,K].T + bias) + residual`` with bias, activation and residual add in the GEMM's
+    epilogue: fp32 up to one rounding to ``x.dtype`` (bf16 / fp16).  ``activation`` is ``None``,
+    ``"relu"``, ``"silu"``, ``"gelu"`` or ``"gelu_tanh"``; ``residual`` is ``[M, N]`` of ``x.dtype``.  Operands as
+    for :func:`gemm` (``K % 8 == 0``).  No reference counterpart (cuBLAS and elementwise kernels there)."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise RuntimeError("gemm_epilogue: expected x [M, K] and w [N, K].")
+    if x.dtype != w.dtype or (residual is not None and residual.dtype != x.dtype):
+        raise RuntimeError("gemm_epilogue: x, w and residual must have the same dtype.")
+    if activation not in _cabi.ACTIVATIONS:
+        raise RuntimeError(f"gemm_epilogue: unknown activation {activation!r}.")
+    m, k = x.shape
+    n = w.shape[0]
+    if residual is not None and tuple(residual.shape) != (m, n):
+        raise RuntimeError(f"gemm_epilogue: residual must be [{m}, {n}], got {list(residual.shape)}.")
+    _cabi.require_cuda("gemm_epilogue", x, w, residual)
+    lib = _cabi.load_library()
+    b = _bias_f32(bias, n, x.device)
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = _launch("npb_gemm_epilogue", lib.npb_gemm_epilogue, x.data_ptr(), w.data_ptr(),
+                     None if b is None else b.data_ptr(), _cabi.ACTIVATIONS[activation],
+                     None if residual is None else residual.data_ptr(), y.data_ptr(), m, n, k,
+                     _cabi.dtype_code(x.dtype), _cabi.stream_ptr())
+    _cabi.check(rc, "gemm_epilogue")
     return y
 
 
