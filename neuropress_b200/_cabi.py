@@ -9,6 +9,7 @@ same situations, e.g. neuropress/kernels/vq_dequant.cu:112-127).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import POINTER, Structure, c_char_p, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
@@ -218,8 +219,22 @@ def dtype_code(dtype: torch.dtype) -> int:
         raise RuntimeError(f"dtype must be bfloat16, float16 or float32, got {dtype}") from None
 
 
+# The current stream's handle without building a Stream object (0.3 us instead of 3.2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, free of charge where that device is the current one."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:

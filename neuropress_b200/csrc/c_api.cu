@@ -117,9 +117,9 @@ int blocks_per_sm(const void* kernel, int threads, size_t smem, int* per_sm) {
   const auto key = std::make_tuple(dev, kernel, smem);
   auto it = cache.find(key);
   if (it == cache.end()) {
-    // opt in as soon as dynamic + (small) static shared memory can pass the 48 KiB default
+    // opt in as soon as dynamic + static shared memory (at most 16 KiB) can pass the 48 KiB default
     size_t& have = opted[std::make_pair(dev, kernel)];
-    if (smem + 1024 > 48 * 1024 && smem > have) {
+    if (smem + 16 * 1024 > 48 * 1024 && smem > have) {
       NPB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
       have = smem;
     }

@@ -473,7 +473,7 @@ def gemm_epilogue(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = 
     lib = _cabi.load_library()
     b = _bias_f32(bias, n, x.device)
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
+    with _cabi.on_device(x.device):
         rc = _launch("npb_gemm_epilogue", lib.npb_gemm_epilogue, x.data_ptr(), w.data_ptr(),
                      None if b is None else b.data_ptr(), _cabi.ACTIVATIONS[activation],
                      None if residual is None else residual.data_ptr(), y.data_ptr(), m, n, k,
@@ -643,7 +643,7 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
     size = lib.npb_q_moe_workspace_bytes(n, top_k, i)
     workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
     x_step, l_step = h * x.element_size(), e * router_logits.element_size()
-    with torch.cuda.device(x.device):
+    with _cabi.on_device(x.device):
         for t0 in range(0, t, n):
             rc = _launch("npb_q_moe", lib.npb_q_moe, x.data_ptr() + t0 * x_step, code,
                          router_logits.data_ptr() + t0 * l_step, logit_code, min(n, t - t0), e, h, i, *structs, top_k,
@@ -758,13 +758,13 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0
         raise RuntimeError(f"token_logprobs: top_n must lie in [0, min(V, {_cabi.LOGPROBS_MAX_TOP})], V > 0.")
     if v > 1 and logits.stride(1) != 1 or r > 1 and logits.stride(0) < v:
         raise RuntimeError("token_logprobs: the rows of logits must be contiguous and must not overlap.")
-    _cabi.require_cuda("token_logprobs", targets, logits[:1])   # rows may be strided
+    # the rows of logits may be strided
+    _cabi.require_cuda("token_logprobs", targets, logits if logits.is_contiguous() else logits[:1])
     lib = _cabi.load_library()
     code = _cabi.dtype_code(logits.dtype)
-    logprob, entropy = torch.empty((2, r), dtype=torch.float32, device=logits.device)
-    top = torch.empty((r, top_n), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((r, top_n), dtype=torch.int64, device=logits.device)
-    with torch.cuda.device(logits.device):
+    logprob, entropy = logits.new_empty((r,), dtype=torch.float32), logits.new_empty((r,), dtype=torch.float32)
+    top, ids = logits.new_empty((r, top_n), dtype=torch.float32), targets.new_empty((r, top_n))
+    with _cabi.on_device(logits.device):
         rc = _launch("npb_token_logprobs", lib.npb_token_logprobs, logits.data_ptr(), logits.stride(0) if r > 1 else v,
                      r, v, code, targets.data_ptr(), int(top_n), logprob.data_ptr(), entropy.data_ptr(),
                      top.data_ptr(), ids.data_ptr(), _cabi.stream_ptr())
