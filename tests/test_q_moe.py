@@ -259,7 +259,7 @@ def test_c_entry_refuses():
         return s
 
     good = dict(x=4096, dtype=1, logits=4096, ldt=2, T=2, E=4, H=64, I=96, gate=weight(), up=weight(), down=weight(),
-                k=2, renorm=1, ws=4096, ws_bytes=2 * 2 * 3 * 80, y=4096)
+                k=2, renorm=1, ws=4096, ws_bytes=2 * 2 * 3 * 160, y=4096)
 
     def call(**change):
         a = {**good, **change}
