@@ -272,9 +272,10 @@ def test_c_entry_refuses():
         assert call(**change) == 1, change
     for change in ({"dtype": 2}, {"ldt": 3}, {"T": 33}, {"E": 513}, {"k": 17, "E": 100}, {"gate": weight(nbits=8)},
                    {"down": weight(g=16)}, {"gate": weight(zp=4096)}, {"gate": weight(g=64)},
-                   {"H": 32800}, {"I": 32800}):
+                   {"H": 16416}, {"I": 16416}):
         assert call(**change) == 2, change
     assert call(H=72) == 3 and call(I=100) == 3 and call(gate=weight(g=96)) == 3
+    assert call(gate=weight(scale=4098)) == 4 and call(down=weight(zp=4098)) == 4
     assert call(x=4098) == 4 and call(ws=4104) == 4 and call(gate=weight(codes=4104)) == 4 and call(y=4097) == 4
     assert call(ws_bytes=good["ws_bytes"] - 1) == 6
     assert call(T=0, x=None) == 0
