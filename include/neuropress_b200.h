@@ -315,9 +315,10 @@ int npb_q_embedding(const int64_t* ids, int64_t T, const npb_q_weight* w, int64_
  *   y[t] = T( sum_{e in S} w_e * D_e ( silu(G_e x[t]) * (U_e x[t]) ) )          fp32 arithmetic
  * x, y [T, H] in dtype (NPB_BF16 / NPB_F16), logits [T, E] in logits_dtype (also NPB_F32).  gate / up
  * are the experts' [I, H] weights stacked to [E * I, H], down the [H, I] weights stacked to
- * [E * H, I]; nbits 4, group_size a multiple of 32, codes 16-byte, scales and zero points 4-byte aligned,
- * gate and up of one group size and both with or both without zero points.  H, I multiples of 32, at most 16384.  Experts with logit -inf are not used, a token
- * whose logits are all -inf yields zeros, one with NaN or +inf yields NaN.  workspace: 16-byte
+ * [E * H, I]; nbits 4, group_size a multiple of 32, codes, scales and zero points 16-byte aligned, gate
+ * and up of one group size and both with or both without zero points.  H, I multiples of 32, at most
+ * 16384.  Experts with logit -inf are not used, a token whose logits are all -inf yields zeros, one
+ * with NaN or +inf yields NaN.  workspace: 16-byte
  * aligned, npb_q_moe_workspace_bytes, not shared by calls that may run at the same time; its
  * content need not be kept or cleared.  Two kernels; the same bits for the same inputs every time.  No
  * reference counterpart: the reference runs every expert's linears by themselves. */

@@ -871,10 +871,32 @@ int q_gemm_fused(const npb_q_weight* w, const void* x, int x_dtype, int64_t M, i
                              : gemm_fused_mt<__half, B_Q4, 0>(x, p, st);
 }
 
+// Row-major [rows, cols] matrix with a box of box_rows x box_cols, elements past the edges read as zero; for the
+// kernels of other files.
+int make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, int64_t rows,
+                       int64_t cols, int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) {
+    set_last_cuda_error(cudaErrorSymbolNotFound, "cuTensorMapEncodeTiled lookup");
+    return NPB_ERR_CUDA;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)cols * elem_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  if (fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    set_last_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    return NPB_ERR_CUDA;
+  }
+  return NPB_OK;
+}
+
 // Reads and clears the device-side give-up record of the GEMM kernels (synchronises).
 int vq_gemm_fused_device_status(int* host_out);  // vq_gemm_fused.cu keeps its own record
 int q_gemv_ring_device_status(int* host_out);    // and so does q_gemv_ring.cu
 int vq_decode_copy_device_status(int* host_out); // and vq_decode_copy.cu
+int q_moe_device_status(int* host_out);          // and q_moe.cu
 
 int gemm_device_status(int* host_out) {
   int v = 0;
@@ -895,6 +917,9 @@ int gemm_device_status(int* host_out) {
   int vs = 0;
   if (int rc = q_gemm_staged_device_status(&vs)) return rc;
   if (v == 0 && vs != 0) v = 40 + vs;
+  int vm = 0;
+  if (int rc = q_moe_device_status(&vm)) return rc;
+  if (v == 0 && vm != 0) v = 50 + vm;
   if (host_out) *host_out = v;
   return v == 0 ? NPB_OK : NPB_ERR_DEVICE_TIMEOUT;
 }

@@ -15,9 +15,10 @@
 // q becomes 1024 + q or, four bits higher in the mantissa, 1024 + 16 q with one bit operation per two
 // codes; the activations that meet the latter are stored divided by 16.  With x' the stored activations
 //   sum_k (q - z) x = D - 1024 sum_k x' - z sum_k x,   D the mma's sum
-// is applied per 32-wide block, with the weight's scale, in fp32.  Activations are stored as fp16 with a power
-// of two per 32-block and token, so their size does not matter: a bf16 or fp16 x loses nothing down to
-// 2^-13 of its block's largest (below that at most 2^-21 of the largest), and h keeps 11 significant bits
+// is applied per 32-wide block, with the weight's scale, in fp32 (the magic's part is the C operand of the first
+// mma).  Activations are stored as fp16 after division by a power of two, one per token for x and one per
+// 32-block and token for h, so their size does not matter: x loses nothing down to 2^-13 (bf16) or 2^-10
+// (fp16) of the token's largest and at most 2^-21 of the largest below that; h keeps 11 significant bits
 // between the kernels, 1/8 of a bf16 half step.
 //
 // The eight columns of an mma are NT = 8 / G tokens times G neighbouring 32-blocks (G = 4, 2, 1): lane (g, t)
@@ -27,12 +28,15 @@
 // sixteen mmas for two 16-row tiles whatever G is (8 cycles of a scheduler's tensor pipe each, measured);
 // G = 4 has the widest loads and the fewest results to scale, G = 1 the most tokens per weight read.
 //
-// Every warp streams its own weights: a ring of steps in shared memory filled by cp.async, so that what is in flight
-// does not depend on registers (register double buffers of the same kernels reached a third of the
-// bandwidth: waiting for one step's loads waits for the next step's too).  Kernel 1 keeps the tokens of its
-// unit (up to NT tokens of one expert) in shared memory in the order of the mma operands and writes h in
-// that order; kernel 2 brings h along with the weights.  An expert with more tokens than a unit is read again
-// (from L2).  Every sum has a fixed order: results do not depend on scheduling.
+// Every warp streams its own weights through a ring of steps in shared memory: codes as TMA boxes of 64 bytes x 16
+// rows with the 64-byte swizzle (no bank conflicts when read, no load instructions, nothing in the L1 path),
+// scales and zero points by cp.async as 16- or 32-byte windows that serve several steps.  What is in flight
+// does not depend on registers: register double buffers of the same kernels reached a third of the bandwidth
+// (waiting for one step's loads waits for the next step's too), and cp.async for the codes left the L1 path
+// 72 % busy.  Kernel 1 keeps the tokens of its unit (up to NT tokens of one expert) in shared memory in the
+// order of the mma operands and writes h in that order; kernel 2 brings h along with the weights.  An expert
+// with more tokens than a unit is read again (from L2).  Every sum has a fixed order: results do not depend
+// on scheduling.  Waits on the TMA barriers are bounded like those of the GEMMs.
 #include <type_traits>
 
 #include "common.cuh"
@@ -40,6 +44,13 @@
 #include "tcgen05.cuh"
 
 namespace npb {
+
+// gemm_tcgen05.cu
+int make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, int64_t rows,
+                       int64_t cols, int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
+
+__device__ int g_moe_status = 0;  // 0 ok; 1, 2: the kernel one of whose waits gave up
+
 namespace {
 
 constexpr int kMaxTokens = 32;   // bits of an expert's token mask
@@ -54,6 +65,7 @@ struct MoeWeight {
   const __half* zp;  // null: symmetric, z = 8
   int group_shift;   // log2 of the 32-blocks per group, or -1: divide
   int group_blocks;
+  int window;        // steps that a window of groups serves
 };
 
 struct MoeParams {
@@ -64,9 +76,10 @@ struct MoeParams {
   MoeWeight gate, up, down;
   uint8_t* h;      // [pair of tokens of a unit][I / 32] records
   void* y;
+  uint64_t wait_ns;
 };
 
-// One 32-block of h of two tokens: 32 stored fp16 values of each (64 bytes), then {f0, f1, c0, c1, s2 of both}.
+// One 32-block of h of two tokens: 32 stored fp16 values of each (64 bytes), then {m0, m1, f0, f1, s2 of both}.
 constexpr int kRecord = 160;
 
 // ---- routing ---------------------------------------------------------------------------------
@@ -184,14 +197,9 @@ __device__ __forceinline__ int group_of(const MoeWeight& w, int blk) {
   return w.group_shift >= 0 ? blk >> w.group_shift : blk / w.group_blocks;
 }
 
-template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool valid = true) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES),
-                 "r"(valid ? BYTES : 0)
-                 : "memory");
+// 16 bytes, of which the first `bytes` are read and the rest is zero.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `pending` (1..3) of the committed groups are under way.
@@ -201,82 +209,67 @@ __device__ __forceinline__ void cp_async_wait(int pending) {
   else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
 
-// One step (four 32-blocks of k) of R 16-row tiles in a warp's ring: per row 64 bytes of codes, the 16-byte pieces
-// permuted so that the reads below are free of bank conflicts, then per row 16 bytes with the scales of the
-// step's groups and, if ASYM, with the zero points.  FAST: one group per block and rows of whole steps, the
-// four values sit in the first eight bytes; otherwise the three words that hold them, which start at an odd
-// fp16 where the row's first group is odd.
-template <int G, int R, bool ASYM, bool FAST>
+// A warp's ring over R 16-row tiles.  A stage holds one step (four 32-blocks of k): per row 64 bytes of codes as TMA's
+// 64-byte swizzle leaves them (16-byte piece c of row r at c ^ (r / 2 mod 4)).  A window holds per row the 16 or 32
+// bytes, from a 16-byte boundary on, with the groups of several steps; there are as many windows as stages: the
+// steps in the ring need no more.  MODE: kOnePerBlock (a group is a block; a step's four values are eight aligned
+// bytes) and kPowerOfTwo (a group is 2^n blocks) take rows of whole 16-byte windows, one for every eight groups;
+// kAny the rest, 32 bytes at a run's first step and every `window`-th after it.
+enum { kAny = 0, kOnePerBlock = 1, kPowerOfTwo = 2 };
+
+template <int G, int R, bool ASYM, int MODE>
 struct Ring {
-  static constexpr int kRows = 16 * R;
-  static constexpr int kScales = kRows * 64, kZeros = kScales + kRows * 16;
-  static constexpr int kBytes = kZeros + (ASYM ? kRows * 16 : 0);
+  static constexpr int kRows = 16 * R, kWindowRow = MODE == kAny ? 32 : 16;
+  static constexpr int kCodes = kRows * 64;
+  static constexpr int kWindow = kRows * kWindowRow * (ASYM ? 2 : 1);
+  static constexpr int kZeros = kRows * kWindowRow;  // of the zero points in a window
 
-  __device__ static int swizzle(int row) { return G == 2 ? (row >> 1 & 1) * 2 : row >> 1 & 3; }
+  // Tile row of lane group g: G = 2 reads half pieces, which needs every other pair of rows in a phase.
+  __device__ static int row_of(int g) { return G == 2 ? (g & 1) | (g & 2) << 1 | (g & 4) >> 1 : g; }
 
-  // Codes of rows 8 i + lane / 4, i < N, to ring rows from `row0` on; `src` points at block 0 of row lane / 4.
-  template <int N>
-  __device__ static void fetch_codes(uint32_t stage, int row0, const uint8_t* src, int s, int n_blk, int lane) {
-    const int c = lane & 3, row = row0 + (lane >> 2);
-    const uint32_t dst = stage + row * 64 + (c ^ swizzle(row)) * 16;  // rows 8 apart have the same swizzle
-    const bool valid = FAST || s * 4 + c < n_blk;
-    src += (s * 4 + c) * 16;
-#pragma unroll
-    for (int i = 0; i < N; ++i) cp_async<16>(dst + i * 512, valid ? src + (int64_t)i * 8 * n_blk * 16 : src - c * 16, valid);
+  // Whether step s brings a window, in a run that began with step `start`.
+  __device__ static bool has_window(const MoeWeight& w, int s, int start) {
+    if (s == start) return true;
+    if (MODE == kOnePerBlock) return (s & 1) == 0;
+    if (MODE == kPowerOfTwo) return (s * 4 & ((8 << w.group_shift) - 1)) == 0;
+    return (s - start) % w.window == 0;
   }
-  // Groups of one row; `at_row` is its first, `total` the number of groups of the matrix.
-  __device__ static void fetch_groups(uint32_t stage, int row, const MoeWeight& w, int64_t at_row, int64_t total, int s) {
-    const uint32_t dst = stage + kScales + row * 16;
-    if constexpr (FAST) {
-      cp_async<8>(dst, w.scale + at_row + s * 4);
-      if (ASYM) cp_async<8>(dst + kRows * 16, w.zp + at_row + s * 4);
-    } else {
-      const int64_t word = (at_row + group_of(w, s * 4)) >> 1;
+  // Place of step s's first group in the window that step w_s brought, for rows that are row_of(g) modulo 8.
+  __device__ static int index_of(const MoeWeight& w, int s, int w_s, int g, int n_group) {
+    if (MODE == kOnePerBlock) return (s & 1) * 4;
+    if (MODE == kPowerOfTwo) return (s * 4 >> w.group_shift) & 7;
+    const int g0 = group_of(w, w_s * 4);
+    return ((row_of(g) * n_group + g0) & 7) + group_of(w, s * 4) - g0;
+  }
+
+  // Windows of rows row0 + lane / PIECES ..: `at` is the first group of ring row 0's step, counted in the matrix of
+  // `total` groups; rows are n_group apart.
+  template <int ROWS>
+  __device__ static void fetch_window(uint32_t window, int row0, const MoeWeight& w, int64_t at, int n_group,
+                                      int64_t total, int lane) {
+    constexpr int PIECES = kWindowRow / 16;
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const bool in = 2 * (word + i) < total;  // total is even: 32 rows to a multiple
-        const int64_t at = in ? 2 * (word + i) : 0;
-        cp_async<4>(dst + i * 4, w.scale + at, in);
-        if (ASYM) cp_async<4>(dst + kRows * 16 + i * 4, w.zp + at, in);
-      }
+    for (int i = 0; i < (ROWS * PIECES + 31) / 32; ++i) {
+      const int row = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
+      if (row >= ROWS) break;
+      const int64_t first = ((at + (int64_t)row * n_group) & ~7ll) + piece * 8;
+      const int left = (int)max((int64_t)0, min((int64_t)8, total - first)) * 2;
+      const uint32_t dst = window + (row0 + row) * kWindowRow + piece * 16;
+      cp_async16(dst, w.scale + (left ? first : 0), left);
+      if (ASYM) cp_async16(dst + kZeros, w.zp + (left ? first : 0), left);
     }
   }
 };
 
-// The values of the four blocks of a step of one row.
-struct GroupReader {
-  uint32_t pick_lo, pick_hi, keep_lo, keep_hi;
-  int shift;
-  // p: 1 if the row's first group of the step is odd; the selectors are the same for every lane
-  __device__ GroupReader(const MoeWeight& w, int s, int n_blk, int p) {
-    shift = p * 16;
-    if (w.group_blocks == 1) {
-      pick_lo = pick_hi = 0;
-    } else {
-      const int first = group_of(w, s * 4);
-      auto byte2 = [&](int j) { return group_of(w, s * 4 + j) != first ? 0x32u : 0x10u; };
-      pick_lo = byte2(0) | byte2(1) << 8;
-      pick_hi = byte2(2) | byte2(3) << 8;
-    }
-    const int left = n_blk - s * 4;  // blocks past the row's last have scale 0
-    keep_lo = left >= 2 ? 0xffffffffu : 0x0000ffffu;
-    keep_hi = left >= 4 ? 0xffffffffu : left >= 3 ? 0x0000ffffu : 0u;
-  }
-  __device__ uint2 operator()(const uint4& v) const {
-    const uint32_t a = __funnelshift_r(v.x, v.y, shift), b = __funnelshift_r(v.y, v.z, shift);
-    uint2 r = make_uint2(a, b);
-    if (pick_lo) r = make_uint2(__byte_perm(a, a, pick_lo), __byte_perm(a, a, pick_hi));
-    return make_uint2(r.x & keep_lo, r.y & keep_hi);
-  }
-};
+__device__ __forceinline__ float half_bits(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)v)); }
 
-// The value of this lane's block of set j.
+// The value of this lane's block of set j among the four of a step.
 template <int G>
 __device__ __forceinline__ float group_value(const uint2& v, int j, int t) {
-  if (G == 4) return __half2float(__ushort_as_half((unsigned short)((t & 2 ? v.y : v.x) >> ((t & 1) * 16))));
-  if (G == 2) return __half2float(__ushort_as_half((unsigned short)((j ? v.y : v.x) >> (t / 2 * 16))));
+  if (G == 4) return half_bits((t & 2 ? v.y : v.x) >> ((t & 1) * 16));
+  if (G == 2) return half_bits((j ? v.y : v.x) >> (t / 2 * 16));
   const uint32_t w = j < 2 ? v.x : v.y;
-  return __half2float(__ushort_as_half((unsigned short)(j & 1 ? w >> 16 : w)));
+  return half_bits(j & 1 ? w >> 16 : w);
 }
 
 // Pair j of a word's codes, j and j + 4, as two fp16 values: 1024 + q (j even) or 1024 + 16 q (j odd).
@@ -300,21 +293,17 @@ __device__ __forceinline__ void a_operands(uint32_t l, uint32_t h, uint32_t (&a)
 }
 
 // ---- stored activations --------------------------------------------------------------------
-// Of one 32-block of two tokens: the powers of two f they were divided by and what to subtract from D for the
-// magic and, for a symmetric weight, for z = 8: floats {f0, f1, c0, c1}; apart from them, {s2 of both}, the sums
-// that a zero point multiplies.
 // The power of two at or below a magnitude (1 for zero, subnormal, inf, NaN).
 __device__ __forceinline__ float power_below(float top) {
   const uint32_t exponent = __float_as_uint(top) >> 23;
   return exponent == 0 || exponent == 255 ? 1.f : __uint_as_float(exponent << 23);
 }
 
-// From the sums of a block's stored values at k = 0, 2 mod 4 (`even`) and 1, 3 mod 4 (`odd`, divided by 16), to
-// this token's place in fc = {f0, f1, c0, c1} and s2.
-__device__ __forceinline__ void put_factors(float* fc, float* s2, float f, float even, float odd, bool asym) {
-  const float sum = even + 16.f * odd, m = 1024.f * (even + odd);
-  fc[0] = f;
-  fc[2] = asym ? m : m + 8.f * sum;
+// A block's m and s2 from the sums of its stored values at k = 0, 2 mod 4 (`even`) and 1, 3 mod 4 (`odd`, divided
+// by 16).
+__device__ __forceinline__ void put_sides(float* m, float* s2, float even, float odd, bool asym) {
+  const float sum = even + 16.f * odd, magic = -1024.f * (even + odd);
+  *m = asym ? magic : magic - 8.f * sum;
   if (s2) *s2 = sum;
 }
 
@@ -330,11 +319,6 @@ __device__ __forceinline__ F2 pack(float a, float b) {
 __device__ __forceinline__ void unpack(const F2& x, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
 }
-__device__ __forceinline__ F2 sub2(const F2& a, const F2& b) {  // a - b
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(b.v), "l"(0xbf800000bf800000ull), "l"(a.v));
-  return r;
-}
 __device__ __forceinline__ F2 mul2(const F2& a, const F2& b) {
   F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
@@ -346,57 +330,58 @@ __device__ __forceinline__ F2 fma2(const F2& a, const F2& b, const F2& c) {
   return r;
 }
 // mma.sync.m16n8k16 fp16; a plain (not volatile) asm, so that the compiler may interleave the tiles
-__device__ __forceinline__ void mma_step(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
-  if (first)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = {c0, c1, c0, c1} + a b
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                         float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 
-// Adds one step to acc[tile][row g, g + 8] (two tokens each).  `stage` is the warp's ring stage; `operand` this
-// lane's part of the first set in B order, BLOCK bytes from block to block (a lane off the diagonal: zeros);
-// `factors` the Factors {f, c} of its two tokens and its block of the first set, FAC bytes from block to block,
-// and `sums` their s2, SUM bytes from block to block.
-template <int G, int R, bool ASYM, bool FAST, int BLOCK, int FAC, int SUM>
-__device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* stage, const uint8_t* operand,
-                                         const uint8_t* factors, const uint8_t* sums, int g, int t, int s, int n_blk,
+// What a block of two tokens brings besides its values: {m0, m1}, minus what the magic (and, for a symmetric
+// weight, z = 8) adds; their powers of two and their sums, each where a kernel has them per block.
+struct Sides {
+  const uint8_t *m, *f, *s2;
+};
+
+// Adds one step to acc[tile][row_of(g), + 8] (two tokens each).  `codes` and `window` are the ring's; `index` the place
+// of the step's first group in this lane's row of the window; `operand` this lane's part of the first set in B
+// order, BLOCK bytes from block to block (a lane off the diagonal: zeros); `sides` belong to its two tokens and its
+// block of the first set, MS bytes from block to block.
+template <int G, int R, bool ASYM, int MODE, bool SCALED, int BLOCK, int MS>
+__device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, const uint8_t* window, int index,
+                                         const uint8_t* operand, const Sides& sides, int g, int t, int s, int n_blk,
                                          const MoeWeight& w) {
-  using Rg = Ring<G, R, ASYM, FAST>;
-  const int sw = Rg::swizzle(g);
+  using Rg = Ring<G, R, ASYM, MODE>;
+  const int r0 = Rg::row_of(g);
+  const uint8_t* at = window + r0 * Rg::kWindowRow + index * 2;
   uint2 sc[R][2], zp[ASYM ? R : 1][2];
-  {
-    const int p = FAST ? 0 : (g * (n_blk / w.group_blocks) + group_of(w, s * 4)) & 1;
-    const GroupReader reader(w, s, n_blk, p);
+  if constexpr (MODE == kOnePerBlock) {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* at = stage + Rg::kScales + (i * 16 + h * 8 + g) * 16;
-        if (FAST) {
-          sc[i][h] = *reinterpret_cast<const uint2*>(at);
-          if (ASYM) zp[ASYM ? i : 0][h] = *reinterpret_cast<const uint2*>(at + Rg::kRows * 16);
-        } else {
-          sc[i][h] = reader(*reinterpret_cast<const uint4*>(at));
-          if (ASYM) zp[ASYM ? i : 0][h] = reader(*reinterpret_cast<const uint4*>(at + Rg::kRows * 16));
-        }
-      }
+    for (int i = 0; i < 2 * R; ++i) {
+      sc[i / 2][i % 2] = *reinterpret_cast<const uint2*>(at + i * 8 * Rg::kWindowRow);
+      if (ASYM) zp[ASYM ? i / 2 : 0][i % 2] = *reinterpret_cast<const uint2*>(at + i * 8 * Rg::kWindowRow + Rg::kZeros);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 4 / G; ++j) {
-    // this lane's G words of the set: piece (block) j G + t / (4 / G) of the row, word t mod 4 / G times G
-    const int piece = ((j * G + t / (4 / G)) ^ sw) * 16 + t % (4 / G) * (4 * G);
+    const int own = s * 4 + j * G + t / (4 / G);  // this lane's block of the set
+    // its G words: 16-byte piece (block) of the row, word t mod 4 / G times G
+    const int piece = ((j * G + t / (4 / G)) ^ (r0 >> 1 & 3)) * 16 + t % (4 / G) * (4 * G);
     uint32_t c[2 * R][G];
 #pragma unroll
     for (int i = 0; i < 2 * R; ++i) {
-      const uint8_t* at = stage + (i * 8 + g) * 64 + piece;
-      if constexpr (G == 4) *reinterpret_cast<uint4*>(c[i]) = *reinterpret_cast<const uint4*>(at);
-      else if constexpr (G == 2) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(at);
-      else c[i][0] = *reinterpret_cast<const uint32_t*>(at);
+      const uint8_t* from = codes + (i * 8 + r0) * 64 + piece;
+      if constexpr (G == 4) *reinterpret_cast<uint4*>(c[i]) = *reinterpret_cast<const uint4*>(from);
+      else if constexpr (G == 2) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(from);
+      else c[i][0] = *reinterpret_cast<const uint32_t*>(from);
     }
+    const float2 m = *reinterpret_cast<const float2*>(sides.m + j * G * MS);
     float d[R][4];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -405,25 +390,34 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* stage, 
       for (int q = 0; q < R; ++q) {
         uint32_t a[2][4];
         a_operands(c[2 * q][i], c[2 * q + 1][i], a);
-        mma_step(d[q], a[0], v.x, v.y, i == 0);
-        mma_step(d[q], a[1], v.z, v.w, false);
+        if (i == 0) mma_from(d[q], a[0], v.x, v.y, m.x, m.y);
+        else mma_add(d[q], a[0], v.x, v.y);
+        mma_add(d[q], a[1], v.z, v.w);
       }
     }
-    const ulonglong2 fc = *reinterpret_cast<const ulonglong2*>(factors + j * G * FAC);
-    const F2 f{fc.x}, m{fc.y};
-    F2 s2{};
-    if (ASYM) s2.v = *reinterpret_cast<const unsigned long long*>(sums + j * G * SUM);
+    F2 f{}, s2{};
+    if (SCALED) f.v = *reinterpret_cast<const unsigned long long*>(sides.f + j * G * MS);
+    if (ASYM) s2.v = *reinterpret_cast<const unsigned long long*>(sides.s2 + j * G * MS);
+    const int group = MODE == kOnePerBlock ? 0 : (group_of(w, own) - group_of(w, s * 4)) * 2;
 #pragma unroll
     for (int q = 0; q < R; ++q)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float scale = group_value<G>(sc[q][h], j, t);
-        F2 v = sub2(pack(d[q][2 * h], d[q][2 * h + 1]), m);
-        if (ASYM) {
-          const float z = -group_value<G>(zp[ASYM ? q : 0][h], j, t);
-          v = fma2(pack(z, z), s2, v);
+        float scale, z = 0.f;
+        if constexpr (MODE == kOnePerBlock) {
+          scale = group_value<G>(sc[q][h], j, t);
+          if (ASYM) z = group_value<G>(zp[ASYM ? q : 0][h], j, t);
+        } else {
+          const uint8_t* from = at + (q * 16 + h * 8) * Rg::kWindowRow + group;
+          const bool in = MODE == kPowerOfTwo || own < n_blk;  // there every step is whole
+          scale = in ? half_bits(*reinterpret_cast<const uint16_t*>(from)) : 0.f;
+          if (ASYM) z = in ? half_bits(*reinterpret_cast<const uint16_t*>(from + Rg::kZeros)) : 0.f;
         }
-        acc[q][h] = fma2(mul2(pack(scale, scale), f), v, acc[q][h]);
+        F2 v = pack(d[q][2 * h], d[q][2 * h + 1]);
+        if (ASYM) v = fma2(pack(-z, -z), s2, v);
+        F2 by = pack(scale, scale);
+        if (SCALED) by = mul2(by, f);
+        acc[q][h] = fma2(by, v, acc[q][h]);
       }
   }
 }
@@ -447,67 +441,91 @@ constexpr int kUpThreads = 512;  // two 16-row tile pairs (gate, up) x eight sli
 constexpr int kUpWarps = kUpThreads / 32;
 constexpr int kUpRows = 32;      // rows of gate and of up per item: one 32-block of h
 constexpr int kUpSlices = 8;
+constexpr int kMaxStages = 4;    // of a ring
 
-// Shared memory of kernel 1 behind the routing: tokens [NT][4 * steps] blocks of 64 bytes (neighbouring rows
-// in the other half of the banks), their Factors, the partial products of two items, 256 bytes of zeros, the
-// warps' rings.
+// Shared memory of kernel 1 behind the routing: the warps' rings (codes, windows), tokens [NT][4 * steps] blocks of
+// 64 bytes (neighbouring rows in the other half of the banks), their m and s2 [NT / 2][blocks], the partial
+// products, 256 bytes of zeros, barriers.
 struct UpLayout {
-  int row, factors, sums, red, zeros, rings, bytes;
-  __host__ __device__ UpLayout(int n_blk, int nt, bool asym, int stage_bytes, int stages) {
+  int windows, x, row, m, s2, red, zeros, bars, bytes;
+  __host__ __device__ UpLayout(int n_blk, int nt, bool asym, int code_bytes, int window_bytes, int stages) {
     const int blocks = (n_blk + 3) / 4 * 4;
+    windows = kUpWarps * stages * code_bytes;
+    x = windows + kUpWarps * stages * window_bytes;
     row = blocks * 64 + 64;
-    factors = row * nt;
-    sums = factors + nt / 2 * blocks * 16;
-    red = sums + (asym ? nt / 2 * blocks * 8 : 0);
-    zeros = red + 2 * kUpSlices * 2 * kUpRows * nt * 4;
-    rings = zeros + 256;
-    bytes = rings + kUpWarps * stages * stage_bytes;
+    m = x + row * nt;
+    s2 = m + nt / 2 * blocks * 8;
+    red = s2 + (asym ? nt / 2 * blocks * 8 : 0);
+    zeros = red + kUpSlices * 2 * kUpRows * nt * 4;
+    bars = zeros + 256;
+    bytes = bars + kUpWarps * kMaxStages * 8 + 1024;  // + alignment of the start
   }
 };
 
-// Stores eight elements of a token (thread j of a row: elements 8 j ...) in the order of the mma operands, and
-// their block's Factors; the lanes of a quad share a block.
+// Stores eight elements of a token (thread j of a row: elements 8 j ...), times `by`, in the order of the mma
+// operands, and their block's sides; the lanes of a quad share a block.
 template <typename T>
-__device__ __forceinline__ void store_operand(const uint4& raw, uint4* to, float* fc, float* s2, bool write, bool asym) {
+__device__ __forceinline__ void store_operand(const uint4& raw, float by, uint4* to, float* m, float* s2, bool write,
+                                              bool asym) {
   const T* v = reinterpret_cast<const T*>(&raw);
-  float top = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(to_f32(v[k])));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const float f = power_below(top), even_by = 1.f / f, odd_by = 0.0625f / f;
   __half2 o[4];
   float even = 0.f, odd = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float by = k & 1 ? odd_by : even_by;
-    o[k] = __floats2half2_rn(to_f32(v[k]) * by, to_f32(v[k + 4]) * by);
+    const float f = k & 1 ? by * 0.0625f : by;
+    o[k] = __floats2half2_rn(to_f32(v[k]) * f, to_f32(v[k + 4]) * f);
     (k & 1 ? odd : even) += __low2float(o[k]) + __high2float(o[k]);
   }
   even = quad_sum(even);
   odd = quad_sum(odd);
   if (write) {
     *to = *reinterpret_cast<const uint4*>(o);
-    if ((threadIdx.x & 3) == 0) put_factors(fc, s2, f, even, odd, asym);
+    if ((threadIdx.x & 3) == 0) put_sides(m, s2, even, odd, asym);
   }
 }
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& raw) {
+  const T* v = reinterpret_cast<const T*>(&raw);
+  float top = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(to_f32(v[k])));
+  return top;
+}
 
-template <int G, bool ASYM, bool FAST>
+struct UpMaps {
+  CUtensorMap gate, up;
+};
+
+template <int G, bool ASYM, int MODE>
 __global__ void __launch_bounds__(kUpThreads, 1)
-moe_up_kernel(const MoeParams p, const int stages) {
+moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int stages) {
   constexpr int NT = 8 / G;
-  using Rg = Ring<G, 2, ASYM, FAST>;
-  extern __shared__ __align__(16) uint8_t dyn[];
+  using Rg = Ring<G, 2, ASYM, MODE>;
+  extern __shared__ uint8_t dyn_raw[];
+  uint8_t* dyn = dyn_raw + ((1024u - (sm100::smem_u32(dyn_raw) & 1023u)) & 1023u);
   __shared__ Routing r;
+  __shared__ uint32_t x_top[NT];     // bits of the largest magnitude of each token
+  __shared__ float x_f[NT];
+  __shared__ int abort_flag;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int n_blk = p.H / 32, n_steps = (n_blk + 3) / 4, blocks = n_steps * 4;
   const int n_group = n_blk / p.gate.group_blocks;
-  const UpLayout at(n_blk, NT, ASYM, Rg::kBytes, stages);
-  float* red = reinterpret_cast<float*>(dyn + at.red);  // [item parity][slice][gate, up][NT][32]
+  const UpLayout at(n_blk, NT, ASYM, Rg::kCodes, Rg::kWindow, stages);
+  float* red = reinterpret_cast<float*>(dyn + at.red);  // [slice][gate, up][NT][32]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + at.bars) + warp * kMaxStages;
   const uint32_t base = sm100::smem_u32(dyn);
   if (tid < 64) reinterpret_cast<uint32_t*>(dyn + at.zeros)[tid] = 0;
+  if (tid == 0) {
+    abort_flag = 0;
+    sm100::tma_prefetch_desc(&maps.gate);
+    sm100::tma_prefetch_desc(&maps.up);
+  }
+  if (lane == 0) {
+    for (int i = 0; i < stages; ++i) sm100::mbar_init(&bars[i], 1);
+    sm100::fence_barrier_init();
+  }
   route<NT>(p, r);
 
   const int tiles = p.I / kUpRows;
@@ -517,71 +535,115 @@ moe_up_kernel(const MoeParams p, const int stages) {
   const int s_first = n_steps * ks / kUpSlices, s_last = n_steps * (ks + 1) / kUpSlices;
   const int lane_blk = t / (4 / G);      // this lane's block of a set
   const bool diag = g / NT == lane_blk;  // it holds the nonzero part of column g
-  const uint8_t* operand = dyn + (diag ? (g % NT) * at.row + lane_blk * 64 + t % (4 / G) * G * 16 : at.zeros);
+  const uint8_t* operand = dyn + (diag ? at.x + (g % NT) * at.row + lane_blk * 64 + t % (4 / G) * G * 16 : at.zeros);
   const int operand_step = diag ? 256 : 0;
-  const int pair_blk = t % (4 / G) * blocks + lane_blk;
-  const uint8_t *factors = dyn + at.factors + pair_blk * 16, *sums = dyn + at.sums + pair_blk * 8;
+  const int pair_blk = (t % (4 / G) * blocks + lane_blk) * 8;
+  const Sides sides{dyn + at.m + pair_blk, nullptr, dyn + at.s2 + pair_blk};
 
   // the warp's ring runs through its steps of all items
-  const int ring = at.rings + warp * stages * Rg::kBytes;
+  const int code_ring = warp * stages * Rg::kCodes, window_ring = at.windows + warp * stages * Rg::kWindow;
   const int64_t total_groups = (int64_t)p.E * p.I * n_group;
-  int f_item = first, f_s = s_first, f_stage = 0;
-  auto fetch = [&] {
-    if (f_item < last && s_first < s_last) {
+  int f_item = s_first < s_last ? first : last, f_s = s_first, f_stage = 0, f_window = 0, f_row = 0;
+  auto f_start = [&] {
+    if (f_item < last) {
       const int u = f_item / tiles;
-      const int64_t row0 = (int64_t)r.unit_expert[u] * p.I + (f_item - u * tiles) * kUpRows + mt * 16;
-      const uint32_t stage = base + ring + f_stage * Rg::kBytes;
-      const int64_t code_row = (row0 + g) * n_blk * 16;
-      Rg::template fetch_codes<2>(stage, 0, p.gate.codes + code_row, f_s, n_blk, lane);
-      Rg::template fetch_codes<2>(stage, 16, p.up.codes + code_row, f_s, n_blk, lane);
-      Rg::fetch_groups(stage, lane, lane < 16 ? p.gate : p.up, (row0 + (lane & 15)) * n_group, total_groups, f_s);
-      if (++f_s == s_last) { f_s = s_first; ++f_item; }
+      f_row = r.unit_expert[u] * p.I + (f_item - u * tiles) * kUpRows + mt * 16;
+    }
+  };
+  f_start();
+  auto fetch = [&] {
+    if (f_item < last) {
+      if (lane == 0) {
+        uint8_t* to = dyn + code_ring + f_stage * Rg::kCodes;
+        sm100::mbar_arrive_expect_tx(&bars[f_stage], Rg::kCodes);
+        sm100::tma_load_2d(to, &maps.gate, &bars[f_stage], f_s * 64, f_row);
+        sm100::tma_load_2d(to + 1024, &maps.up, &bars[f_stage], f_s * 64, f_row);
+      }
+      if (Rg::has_window(p.gate, f_s, s_first)) {
+        const uint32_t to = base + window_ring + f_window * Rg::kWindow;
+        if (++f_window == stages) f_window = 0;
+        const int64_t group = (int64_t)f_row * n_group + group_of(p.gate, f_s * 4);
+        Rg::template fetch_window<16>(to, 0, p.gate, group, n_group, total_groups, lane);
+        Rg::template fetch_window<16>(to, 16, p.up, group, n_group, total_groups, lane);
+      }
+      if (++f_s == s_last) { f_s = s_first; ++f_item; f_start(); }
       if (++f_stage == stages) f_stage = 0;
     }
     cp_async_commit();
   };
   for (int i = 0; i < stages; ++i) fetch();
 
-  int unit = -1, n = 0, stage = 0;
+  int unit = -1, n = 0, stage = 0, window = -1;  // of the step at hand
+  uint32_t parity = 0;
+  bool ok = true;
   for (int item = first; item < last; ++item) {
     const int u = item / tiles, i0 = (item - u * tiles) * kUpRows;
     const int e = r.unit_expert[u];
     if (u != unit) {
-      if (unit >= 0) __syncthreads();  // everybody is through with the unit before
+      if (tid < NT) x_top[tid] = 0;
+      __syncthreads();  // everybody is through with the unit before
       unit = u;
-      uint32_t m = r.unit_mask[u];
-      n = __popc(m);
-      // the unit's tokens: a thread takes eight elements (columns of an mma past the last token hold what was
-      // there: nothing reads their sums)
+      const uint32_t mask = r.unit_mask[u];
+      n = __popc(mask);
+      // the unit's tokens, a thread takes eight elements (columns of an mma past the last token hold what was there:
+      // nothing reads their sums): the largest magnitude, then the stored values
 #pragma unroll 1
-      for (int i = 0; i < n; ++i, m &= m - 1) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.x) + (int64_t)(__ffs(m) - 1) * (n_blk * 4);
-        for (int j0 = 0; j0 < blocks * 4; j0 += kUpThreads) {  // whole warps
-          const int j = j0 + tid;
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (j < n_blk * 4) raw = __ldg(src + j);
-          uint4* to = reinterpret_cast<uint4*>(dyn + i * at.row + j * 16);
-          const int pb = i / 2 * blocks + (j >> 2);
-          float* fc = reinterpret_cast<float*>(dyn + at.factors) + pb * 4 + (i & 1);
-          float* s2 = ASYM ? reinterpret_cast<float*>(dyn + at.sums) + pb * 2 + (i & 1) : nullptr;
-          if (p.dtype == NPB_BF16) store_operand<__nv_bfloat16>(raw, to, fc, s2, j < blocks * 4, ASYM);
-          else store_operand<__half>(raw, to, fc, s2, j < blocks * 4, ASYM);
+      for (int pass = 0; pass < 2; ++pass) {
+        uint32_t m = mask;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i, m &= m - 1) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.x) + (int64_t)(__ffs(m) - 1) * (n_blk * 4);
+          float f = 1.f;
+          if (pass) {
+            f = power_below(__uint_as_float(x_top[i]));
+            if (tid == 0) x_f[i] = f;
+          }
+          float top = 0.f;
+          for (int j0 = 0; j0 < blocks * 4; j0 += kUpThreads) {  // whole warps
+            const int j = j0 + tid;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (j < n_blk * 4) raw = __ldg(src + j);
+            if (pass == 0) {
+              top = fmaxf(top, p.dtype == NPB_BF16 ? largest<__nv_bfloat16>(raw) : largest<__half>(raw));
+              continue;
+            }
+            uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
+            const int pb = (i / 2 * blocks + (j >> 2)) * 2 + (i & 1);
+            float* to_m = reinterpret_cast<float*>(dyn + at.m) + pb;
+            float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + pb : nullptr;
+            const bool write = j < blocks * 4;
+            if (p.dtype == NPB_BF16) store_operand<__nv_bfloat16>(raw, 1.f / f, to, to_m, to_s2, write, ASYM);
+            else store_operand<__half>(raw, 1.f / f, to, to_m, to_s2, write, ASYM);
+          }
+          if (pass == 0) {
+            const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+            if (lane == 0) atomicMax(&x_top[i], bits);
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
     }
     F2 acc[2][2] = {};
+    int w_s = 0;
     for (int s = s_first; s < s_last; ++s) {
+      ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
       cp_async_wait(stages - 1);
       __syncwarp();
-      add_step<G, 2, ASYM, FAST, 64, 16, 8>(acc, dyn + ring + stage * Rg::kBytes, operand + s * operand_step,
-                                            factors + s * 64, sums + s * 32, g, t, s, n_blk, p.gate);
+      if (Rg::has_window(p.gate, s, s_first)) {
+        if (++window == stages) window = 0;
+        w_s = s;
+      }
+      const int index = Rg::index_of(p.gate, s, w_s, g, n_group);
+      const Sides here{sides.m + s * 32, nullptr, sides.s2 + s * 32};
+      add_step<G, 2, ASYM, MODE, false, 64, 8>(acc, dyn + code_ring + stage * Rg::kCodes,
+                                               dyn + window_ring + window * Rg::kWindow, index, operand + s * operand_step, here, g, t, s, n_blk, p.gate);
       __syncwarp();
       fetch();
-      if (++stage == stages) stage = 0;
+      if (++stage == stages) { stage = 0; parity ^= 1; }
     }
+    __syncthreads();  // the item before is read
     // the blocks of a set, then the slices of K
-    float* part = red + ((item & 1) * kUpSlices + ks) * 2 * NT * kUpRows;
+    float* part = red + ks * 2 * NT * kUpRows;
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -591,7 +653,7 @@ moe_up_kernel(const MoeParams p, const int stages) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float q = block_sum<G>(v[c]);
-          if (t < 4 / G) part[(w * NT + 2 * t + c) * kUpRows + mt * 16 + g + h * 8] = q;
+          if (t < 4 / G) part[(w * NT + 2 * t + c) * kUpRows + mt * 16 + Rg::row_of(g) + h * 8] = q;
         }
       }
     __syncthreads();
@@ -599,10 +661,12 @@ moe_up_kernel(const MoeParams p, const int stages) {
       float gate = 0.f, up = 0.f;
 #pragma unroll
       for (int k = 0; k < kUpSlices; ++k) {
-        const float* from = red + (((item & 1) * kUpSlices + k) * 2 * NT + warp) * kUpRows + lane;
+        const float* from = red + (k * 2 * NT + warp) * kUpRows + lane;
         gate += from[0];
         up += from[NT * kUpRows];
       }
+      gate *= x_f[warp];
+      up *= x_f[warp];
       uint32_t m = r.unit_mask[u];
       for (int i = 0; i < warp; ++i) m &= m - 1;
       const int token = __ffs(m) - 1;
@@ -621,12 +685,17 @@ moe_up_kernel(const MoeParams p, const int stages) {
       reinterpret_cast<__half*>(rec)[(warp & 1) * 32 + (lane & 24) + (lane & 3) * 2 + ((lane >> 2) & 1)] = v;
       if (lane == 0) {
         float* to = reinterpret_cast<float*>(rec + 128) + (warp & 1);
-        put_factors(to, to + 4, f, even, odd, p.down.zp != nullptr);
+        put_sides(to, to + 4, even, odd, p.down.zp != nullptr);
+        to[2] = f;
       }
     }
-    // the next item writes the other half of `red`, the one after it only behind the next barrier
   }
+  if (!ok) atomicExch(&g_moe_status, 1);
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!ok) {  // let copies that were issued land before the shared memory is released
+    const uint64_t t0 = sm100::global_timer_ns();
+    while (sm100::global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
 }
 
 // ---- kernel 2: down product and the sum over experts ----------------------------------------------
@@ -636,16 +705,17 @@ constexpr int kDownTiles = 4;                 // 16-row tiles per warp: h is bro
 constexpr int kDownRows = 16 * kDownTiles;    // output rows per cluster
 constexpr int kDownSplit = 4;                 // CTAs of a cluster: each takes a share of the (unit, step) sequence
 
-// Shared memory of kernel 2 behind the routing: per warp the partial sums [T][64] and a ring of steps, each followed
-// by h records [NT / 2][4]; then zeros that cover the reach of a step's operands.
+// Shared memory of kernel 2 behind the routing: per warp a ring of codes, a ring of windows and h records
+// [NT / 2][4], the partial sums [T][64]; then zeros that cover the reach of a step's operands, barriers.
 struct DownLayout {
-  int sums, stage, warp, zeros, bytes;
-  __host__ __device__ DownLayout(int T, int nt, int stage_bytes, int stages) {
-    sums = T * kDownRows * 4;
-    stage = stage_bytes + nt / 2 * 4 * kRecord;
-    warp = sums + stages * stage;
-    zeros = warp * kDownWarps;
-    bytes = zeros + 4 * kRecord;
+  int rest, stage, windows, warp_rest, zeros, bars, bytes;
+  __host__ __device__ DownLayout(int T, int nt, int code_bytes, int window_bytes, int stages) {
+    rest = kDownWarps * stages * code_bytes;
+    stage = window_bytes + nt / 2 * 4 * kRecord;
+    warp_rest = stages * stage + T * kDownRows * 4;
+    zeros = rest + kDownWarps * warp_rest;
+    bars = zeros + 4 * kRecord;
+    bytes = bars + kDownWarps * kMaxStages * 8 + 1024;
   }
 };
 
@@ -655,24 +725,39 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-template <int G, bool ASYM, bool FAST>
+template <int G, bool ASYM, int MODE>
 __global__ void __cluster_dims__(kDownSplit, 1, 1) __launch_bounds__(kDownThreads, G == 1 ? 1 : 2)
-moe_down_kernel(const MoeParams p, const int stages) {
+moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, const int stages) {
   constexpr int NT = 8 / G;
-  using Rg = Ring<G, kDownTiles, ASYM, FAST>;
-  extern __shared__ __align__(16) uint8_t dyn[];
+  using Rg = Ring<G, kDownTiles, ASYM, MODE>;
+  extern __shared__ uint8_t dyn_raw[];
+  uint8_t* dyn = dyn_raw + ((1024u - (sm100::smem_u32(dyn_raw) & 1023u)) & 1023u);
   __shared__ Routing r;
+  __shared__ int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int n_blk = p.I / 32, n_steps = (n_blk + 3) / 4, n_group = n_blk / p.down.group_blocks;
   const int rank = (int)sm100::cluster_ctarank();
   const int j0 = blockIdx.x / kDownSplit * kDownRows;
   const int rows_left = min(kDownRows, p.H - j0);  // 32 in the last cluster of an odd H / 32
-  const DownLayout at(p.T, NT, Rg::kBytes, stages);
+  const DownLayout at(p.T, NT, Rg::kCodes, Rg::kWindow, stages);
   const uint32_t base = sm100::smem_u32(dyn);
-  float* sums = reinterpret_cast<float*>(dyn + warp * at.warp);  // [T][64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + at.bars) + warp * kMaxStages;
+  const int code_ring = warp * stages * Rg::kCodes, rest_ring = at.rest + warp * at.warp_rest;
+  auto sums_of = [&](int w) {
+    return reinterpret_cast<float*>(dyn + at.rest + w * at.warp_rest + stages * at.stage);  // [T][64]
+  };
+  float* sums = sums_of(warp);
   for (int i = lane; i < p.T * kDownRows; i += 32) sums[i] = 0.f;
   for (int i = tid; i < kRecord; i += kDownThreads) reinterpret_cast<uint32_t*>(dyn + at.zeros)[i] = 0;
+  if (tid == 0) {
+    abort_flag = 0;
+    sm100::tma_prefetch_desc(&map);
+  }
+  if (lane == 0) {
+    for (int i = 0; i < stages; ++i) sm100::mbar_init(&bars[i], 1);
+    sm100::fence_barrier_init();
+  }
   route<NT>(p, r);
 
   // (unit, step) pairs in a row, an equal share of consecutive ones per warp of the cluster
@@ -681,35 +766,41 @@ moe_down_kernel(const MoeParams p, const int stages) {
   const int first = (int)(total * share / shares), last = (int)(total * (share + 1) / shares);
   const int lane_blk = t / (4 / G);
   const bool diag = g / NT == lane_blk;
-  const int ring = warp * at.warp + at.sums;
-  const uint8_t* operand = dyn + (diag ? ring + Rg::kBytes + (g % NT / 2 * 4 + lane_blk) * kRecord + (g & 1) * 64 +
+  const uint8_t* operand = dyn + (diag ? rest_ring + Rg::kWindow + (g % NT / 2 * 4 + lane_blk) * kRecord + (g & 1) * 64 +
                                              t % (4 / G) * G * 16
                                        : at.zeros);
   const int operand_stage = diag ? at.stage : 0;
-  const uint8_t* factors = dyn + ring + Rg::kBytes + (t % (4 / G) * 4 + lane_blk) * kRecord + 128;
+  const uint8_t* sides = dyn + rest_ring + Rg::kWindow + (t % (4 / G) * 4 + lane_blk) * kRecord + 128;
 
   const int64_t total_groups = (int64_t)p.E * p.H * n_group;
-  int f_at = first, f_u = first / n_steps, f_s = first - f_u * n_steps, f_stage = 0;
+  const int first_u = first / n_steps, first_s = first - first_u * n_steps;
+  // a run is what the warp does of one unit
+  auto has_window = [&](int q, int s) { return Rg::has_window(p.down, s, q - s < first ? first_s : 0); };
+  int f_at = first, f_u = first_u, f_s = first_s, f_stage = 0, f_window = 0;
   auto fetch_weights = [&] {
-    const int64_t row0 = (int64_t)r.unit_expert[f_u] * p.H + j0;
-    const uint32_t to = base + ring + f_stage * at.stage;
-    Rg::template fetch_codes<4>(to, 0, p.down.codes + (row0 + g) * n_blk * 16, f_s, n_blk, lane);
-    if (rows_left == kDownRows)
-      Rg::template fetch_codes<4>(to, 32, p.down.codes + (row0 + 32 + g) * n_blk * 16, f_s, n_blk, lane);
-#pragma unroll
-    for (int i = 0; i < kDownRows; i += 32)
-      if (i < rows_left) Rg::fetch_groups(to, i + lane, p.down, (row0 + i + lane) * n_group, total_groups, f_s);
+    const int row0 = r.unit_expert[f_u] * p.H + j0;
+    if (lane == 0) {
+      sm100::mbar_arrive_expect_tx(&bars[f_stage], Rg::kCodes);
+      sm100::tma_load_2d(dyn + code_ring + f_stage * Rg::kCodes, &map, &bars[f_stage], f_s * 64, row0);
+    }
+    if (has_window(f_at, f_s)) {
+      Rg::template fetch_window<kDownRows>(base + rest_ring + f_window * at.stage, 0, p.down,
+                                           (int64_t)row0 * n_group + group_of(p.down, f_s * 4), n_group, total_groups,
+                                           lane);
+      if (++f_window == stages) f_window = 0;
+    }
   };
   auto fetch_records = [&] {  // blocks 4 f_s .. + 4 of the unit's tokens; zeros past n_blk
     constexpr int kPieces = kRecord / 16;
     const uint8_t* rec = p.h + ((int64_t)r.unit_slot[f_u] * n_blk + f_s * 4) * kRecord;
     const int pieces = (__popc(r.unit_mask[f_u]) + 1) / 2 * 4 * kPieces;
-    const uint32_t to = base + ring + f_stage * at.stage + Rg::kBytes;
+    const uint32_t to = base + rest_ring + f_stage * at.stage + Rg::kWindow;
 #pragma unroll
     for (int c0 = 0; c0 < NT / 2 * 4 * kPieces; c0 += 32) {
       const int c = c0 + lane, pair = c / (4 * kPieces), rest = c - pair * 4 * kPieces;
       const bool valid = f_s * 4 + rest / kPieces < n_blk;
-      if (c < pieces) cp_async<16>(to + c * 16, valid ? rec + (int64_t)pair * n_blk * kRecord + rest * 16 : p.h, valid);
+      if (c < pieces)
+        cp_async16(to + c * 16, valid ? rec + (int64_t)pair * n_blk * kRecord + rest * 16 : p.h, valid ? 16 : 0);
     }
   };
   auto advance = [&] {
@@ -736,7 +827,7 @@ moe_down_kernel(const MoeParams p, const int stages) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float q = block_sum<G>(v[c]);
-          if (t < 4 / G && token[c] >= 0) sums[token[c] * kDownRows + w * 16 + h * 8 + g] += q;
+          if (t < 4 / G && token[c] >= 0) sums[token[c] * kDownRows + w * 16 + h * 8 + Rg::row_of(g)] += q;
         }
         acc[w][h] = F2{0ull};
       }
@@ -744,32 +835,40 @@ moe_down_kernel(const MoeParams p, const int stages) {
   };
 
   // the first weights are under way before kernel 1 ends; h exists only after it
-  const int f0 = f_at, u0 = f_u, s0 = f_s;
   for (int i = 0; i < stages; ++i) {
     if (f_at < last) fetch_weights();
     advance();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  f_at = f0;
-  f_u = u0;
-  f_s = s0;
+  f_at = first;
+  f_u = first_u;
+  f_s = first_s;
   f_stage = 0;
   for (int i = 0; i < stages; ++i) {
     if (f_at < last) fetch_records();
     advance();
   }
-  int c_u = first / n_steps, c_s = first - c_u * n_steps, stage = 0;
+  int c_u = first_u, c_s = first_s, stage = 0, window = -1, w_s = 0;
+  uint32_t parity = 0;
+  bool ok = true;
   for (int q = first; q < last; ++q) {
     if (c_u != unit) {
       flush();
       unit = c_u;
     }
+    ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
     cp_async_wait(stages - 1);
     __syncwarp();
-    const uint8_t* f = factors + stage * at.stage;
-    add_step<G, kDownTiles, ASYM, FAST, kRecord, kRecord, kRecord>(acc, dyn + ring + stage * at.stage,
-                                                                   operand + stage * operand_stage, f, f + 16, g, t, c_s,
-                                                                   n_blk, p.down);
+    if (has_window(q, c_s)) {
+      if (++window == stages) window = 0;
+      w_s = c_s;
+    }
+    const int index = Rg::index_of(p.down, c_s, w_s, g, n_group);
+    const uint8_t* side = sides + stage * at.stage;
+    add_step<G, kDownTiles, ASYM, MODE, true, kRecord, kRecord>(acc, dyn + code_ring + stage * Rg::kCodes,
+                                                                dyn + rest_ring + window * at.stage, index, operand + stage * operand_stage,
+                                                                Sides{side, side + 8, side + 16}, g, t, c_s, n_blk,
+                                                                p.down);
     __syncwarp();
     if (f_at < last) {
       fetch_weights();
@@ -777,17 +876,23 @@ moe_down_kernel(const MoeParams p, const int stages) {
     }
     advance();
     if (++c_s == n_steps) { c_s = 0; ++c_u; }
-    if (++stage == stages) stage = 0;
+    if (++stage == stages) { stage = 0; parity ^= 1; }
   }
   flush();
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!ok) {
+    atomicExch(&g_moe_status, 2);
+    const uint64_t t0 = sm100::global_timer_ns();
+    while (sm100::global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
   __syncthreads();
   // the warps of the CTA (into warp 0's sums), then the CTAs of the cluster: each finishes a quarter of the rows
+  float* cta_sums = sums_of(0);
   for (int i = tid; i < p.T * kDownRows; i += kDownThreads) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDownWarps; ++w) v += reinterpret_cast<const float*>(dyn + w * at.warp)[i];
-    reinterpret_cast<float*>(dyn)[i] = v;
+    for (int w = 0; w < kDownWarps; ++w) v += sums_of(w)[i];
+    cta_sums[i] = v;
   }
   __syncwarp();
   sm100::cluster_sync_all();
@@ -797,7 +902,7 @@ moe_down_kernel(const MoeParams p, const int stages) {
     float v = 0.f;
 #pragma unroll
     for (int c = 0; c < kDownSplit; ++c)
-      v += ld_cluster_f32(sm100::map_to_cta(base + (token * kDownRows + row) * 4, c));
+      v += ld_cluster_f32(sm100::map_to_cta(sm100::smem_u32(cta_sums) + (token * kDownRows + row) * 4, c));
     if (row >= rows_left) continue;
     const int64_t to = (int64_t)token * p.H + j0 + row;
     if (p.dtype == NPB_BF16) static_cast<__nv_bfloat16*>(p.y)[to] = from_f32<__nv_bfloat16>(v);
@@ -808,90 +913,120 @@ moe_down_kernel(const MoeParams p, const int stages) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------
-// One group per block, rows of whole steps, eight-byte words of groups.
-bool is_fast(const MoeWeight& w, int n_blk) {
-  return n_blk % 4 == 0 && w.group_blocks == 1 && aligned_to(w.scale, 8) && aligned_to(w.zp, 8);
+int mode_of(const MoeWeight& w, int n_blk) {
+  if (w.group_shift < 0 || (n_blk / w.group_blocks) % 8 != 0) return kAny;
+  return w.group_blocks == 1 ? kOnePerBlock : kPowerOfTwo;
 }
 
-constexpr int kMaxStages = 4;
+// Codes [rows, bytes of a row] in boxes of 64 bytes x box_rows.
+int make_code_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int64_t row_bytes, int box_rows) {
+  return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, row_bytes, box_rows, 64,
+                            CU_TENSOR_MAP_SWIZZLE_64B);
+}
 
 // Ring stages that fit next to the rest (2..4; 0: not even two do).
 template <typename Bytes>
 int pick_stages(Bytes bytes, int ctas_per_sm) {
   const int cap = ctas_per_sm == 1 ? max_dynamic_smem() : (max_dynamic_smem() - 1024) / ctas_per_sm - 1024;
   int stages = kMaxStages;
-  while (stages >= 2 && bytes(stages) + (int)sizeof(Routing) + 64 > cap) --stages;
+  while (stages >= 2 && bytes(stages) + (int)sizeof(Routing) + 256 > cap) --stages;
   return stages >= 2 ? stages : 0;
 }
 
-template <int G, bool ASYM, bool FAST>
-int up_stages(const MoeParams& p) {
-  return pick_stages([&](int n) { return UpLayout(p.H / 32, 8 / G, ASYM, Ring<G, 2, ASYM, FAST>::kBytes, n).bytes; }, 1);
+int window_bytes(int rows, bool asym, int mode) { return rows * (mode == kAny ? 32 : 16) * (asym ? 2 : 1); }
+
+int up_bytes(const MoeParams& p, int g, int stages) {
+  return UpLayout(p.H / 32, 8 / g, p.gate.zp != nullptr, 32 * 64,
+                  window_bytes(32, p.gate.zp != nullptr, mode_of(p.gate, p.H / 32)), stages).bytes;
+}
+int up_stages(const MoeParams& p, int g) {
+  return pick_stages([&](int n) { return up_bytes(p, g, n); }, 1);
+}
+int down_bytes(const MoeParams& p, int g, int stages) {
+  return DownLayout(p.T, 8 / g, kDownRows * 64,
+                    window_bytes(kDownRows, p.down.zp != nullptr, mode_of(p.down, p.I / 32)), stages).bytes;
+}
+int down_stages(const MoeParams& p, int g) {
+  auto bytes = [&](int n) { return down_bytes(p, g, n); };
+  const int two = g == 1 ? 0 : pick_stages(bytes, 2);  // two CTAs on an SM where they fit
+  return two ? two : pick_stages(bytes, 1);
 }
 
-template <int G, bool ASYM, bool FAST>
+template <int G, bool ASYM, int MODE>
 int launch_up(const MoeParams& p, cudaStream_t st) {
-  auto kern = moe_up_kernel<G, ASYM, FAST>;
-  const int stages = up_stages<G, ASYM, FAST>(p);
-  if (stages == 0) return NPB_ERR_TOO_LARGE;
-  const size_t smem = UpLayout(p.H / 32, 8 / G, ASYM, Ring<G, 2, ASYM, FAST>::kBytes, stages).bytes;
+  auto kern = moe_up_kernel<G, ASYM, MODE>;
+  const int stages = up_stages(p, G), smem = up_bytes(p, G, stages);
   int per_sm = 0;
   if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kUpThreads, smem, &per_sm)) return rc;
   if (per_sm < 1) return NPB_ERR_TOO_LARGE;
+  UpMaps maps;
+  if (int rc = make_code_map(&maps.gate, p.gate.codes, (int64_t)p.E * p.I, p.H / 2, 16)) return rc;
+  if (int rc = make_code_map(&maps.up, p.up.codes, (int64_t)p.E * p.I, p.H / 2, 16)) return rc;
   const int64_t active = p.T * p.top_k < p.E ? p.T * p.top_k : p.E;
   const int64_t most = active * (p.I / kUpRows), slots = (int64_t)sm_count() * per_sm;
-  kern<<<(unsigned)(most < slots ? most : slots), kUpThreads, smem, st>>>(p, stages);
+  kern<<<(unsigned)(most < slots ? most : slots), kUpThreads, smem, st>>>(maps, p, stages);
   NPB_LAUNCH_CHECK();
   return NPB_OK;
 }
 
-template <int G, bool ASYM, bool FAST>
+template <int G, bool ASYM, int MODE>
 int launch_down(const MoeParams& p, cudaStream_t st) {
-  auto kern = moe_down_kernel<G, ASYM, FAST>;
-  auto bytes = [&](int n) { return DownLayout(p.T, 8 / G, Ring<G, kDownTiles, ASYM, FAST>::kBytes, n).bytes; };
-  int stages = pick_stages(bytes, 2);
-  if (stages == 0) stages = pick_stages(bytes, 1);
-  if (stages == 0) return NPB_ERR_TOO_LARGE;
+  auto kern = moe_down_kernel<G, ASYM, MODE>;
+  const int stages = down_stages(p, G), smem = down_bytes(p, G, stages);
   int per_sm = 0;
-  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kDownThreads, bytes(stages), &per_sm)) return rc;
+  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kDownThreads, smem, &per_sm)) return rc;
   if (per_sm < 1) return NPB_ERR_TOO_LARGE;
+  CUtensorMap map;
+  if (int rc = make_code_map(&map, p.down.codes, (int64_t)p.E * p.H, p.I / 2, kDownRows)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((p.H + kDownRows - 1) / kDownRows * kDownSplit));
   cfg.blockDim = dim3(kDownThreads);
-  cfg.dynamicSmemBytes = bytes(stages);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, stages));
+  NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, map, p, stages));
   NPB_LAUNCH_CHECK();
   return NPB_OK;
 }
 
+template <int G, bool ASYM>
+int launch_up_mode(const MoeParams& p, cudaStream_t st) {
+  switch (mode_of(p.gate, p.H / 32)) {
+    case kOnePerBlock: return launch_up<G, ASYM, kOnePerBlock>(p, st);
+    case kPowerOfTwo: return launch_up<G, ASYM, kPowerOfTwo>(p, st);
+    default: return launch_up<G, ASYM, kAny>(p, st);
+  }
+}
+template <int G, bool ASYM>
+int launch_down_mode(const MoeParams& p, cudaStream_t st) {
+  switch (mode_of(p.down, p.I / 32)) {
+    case kOnePerBlock: return launch_down<G, ASYM, kOnePerBlock>(p, st);
+    case kPowerOfTwo: return launch_down<G, ASYM, kPowerOfTwo>(p, st);
+    default: return launch_down<G, ASYM, kAny>(p, st);
+  }
+}
 template <int G>
 int launch(const MoeParams& p, cudaStream_t st) {
-  const bool fast_up = is_fast(p.gate, p.H / 32) && is_fast(p.up, p.H / 32), fast_down = is_fast(p.down, p.I / 32);
-  int rc;
-  if (p.gate.zp) rc = fast_up ? launch_up<G, true, true>(p, st) : launch_up<G, true, false>(p, st);
-  else rc = fast_up ? launch_up<G, false, true>(p, st) : launch_up<G, false, false>(p, st);
-  if (rc) return rc;
-  if (p.down.zp) return fast_down ? launch_down<G, true, true>(p, st) : launch_down<G, true, false>(p, st);
-  return fast_down ? launch_down<G, false, true>(p, st) : launch_down<G, false, false>(p, st);
+  if (int rc = p.gate.zp ? launch_up_mode<G, true>(p, st) : launch_up_mode<G, false>(p, st)) return rc;
+  return p.down.zp ? launch_down_mode<G, true>(p, st) : launch_down_mode<G, false>(p, st);
 }
 
 int launch_tokens(const MoeParams& p, cudaStream_t st) {
-  // an expert has at most T tokens; a unit's tokens have to fit the shared memory of kernel 1 (ASYM's larger ring)
-  if (p.T > 4 && up_stages<1, true, false>(p)) return launch<1>(p, st);
-  if (p.T > 2 && up_stages<2, true, false>(p)) return launch<2>(p, st);
-  return launch<4>(p, st);
+  // an expert has at most T tokens; both kernels need two stages next to a unit's tokens
+  auto fits = [&](int g) { return up_stages(p, g) && down_stages(p, g); };
+  if (p.T > 4 && fits(1)) return launch<1>(p, st);
+  if (p.T > 2 && fits(2)) return launch<2>(p, st);
+  return fits(4) ? launch<4>(p, st) : NPB_ERR_TOO_LARGE;
 }
 
 int make_weight(const npb_q_weight* w, int64_t N, int64_t K, MoeWeight* out) {
   if (int rc = validate_q(w, N, K)) return rc;
   if (w->nbits != 4 || w->group_size % 32 != 0) return NPB_ERR_UNSUPPORTED;
-  if (!aligned_to(w->codes, 16) || !aligned_to(w->scale, 4) || !aligned_to(w->zero_point, 4)) return NPB_ERR_ALIGNMENT;
+  if (!aligned_to(w->codes, 16) || !aligned_to(w->scale, 16) || !aligned_to(w->zero_point, 16)) return NPB_ERR_ALIGNMENT;
   out->codes = w->codes;
   out->scale = static_cast<const __half*>(w->scale);
   out->zp = static_cast<const __half*>(w->zero_point);
@@ -899,10 +1034,23 @@ int make_weight(const npb_q_weight* w, int64_t N, int64_t K, MoeWeight* out) {
   out->group_shift = -1;
   for (int s = 0; s < 16; ++s)
     if (out->group_blocks == 1 << s) out->group_shift = s;
+  // the last group of the last step lies at most eight groups behind the first, which lies at most seven behind
+  // the window's start: sixteen values hold them
+  out->window = out->group_blocks >= 4 ? 8 : 2 * out->group_blocks;
   return NPB_OK;
 }
 
 }  // namespace
+
+// Reads and clears the give-up record (npb_gemm_device_status collects it).
+int q_moe_device_status(int* host_out) {
+  NPB_CUDA_TRY(cudaMemcpyFromSymbol(host_out, g_moe_status, sizeof(int)));
+  if (*host_out != 0) {
+    const int zero = 0;
+    NPB_CUDA_TRY(cudaMemcpyToSymbol(g_moe_status, &zero, sizeof(int)));
+  }
+  return NPB_OK;
+}
 
 int64_t q_moe_workspace_bytes(int64_t T, int top_k, int64_t I) {
   if (T < 0 || top_k <= 0 || I <= 0 || T > kMaxTokens || top_k > kMaxTopK || I % 32 != 0) return 0;
@@ -938,6 +1086,7 @@ int q_moe(const void* x, int dtype, const void* logits, int logits_dtype, int64_
   p.renormalize = renormalize != 0;
   p.h = static_cast<uint8_t*>(workspace);
   p.y = y;
+  p.wait_ns = wait_limit_ns();
   return launch_tokens(p, st);
 }
 

@@ -275,7 +275,7 @@ def test_c_entry_refuses():
                    {"H": 16416}, {"I": 16416}):
         assert call(**change) == 2, change
     assert call(H=72) == 3 and call(I=100) == 3 and call(gate=weight(g=96)) == 3
-    assert call(gate=weight(scale=4098)) == 4 and call(down=weight(zp=4098)) == 4
+    assert call(gate=weight(scale=4104)) == 4 and call(down=weight(zp=4104)) == 4
     assert call(x=4098) == 4 and call(ws=4104) == 4 and call(gate=weight(codes=4104)) == 4 and call(y=4097) == 4
     assert call(ws_bytes=good["ws_bytes"] - 1) == 6
     assert call(T=0, x=None) == 0
