@@ -15,8 +15,7 @@
 // q becomes 1024 + q or, four bits higher in the mantissa, 1024 + 16 q with one bit operation per two
 // codes; the activations that meet the latter are stored divided by 16.  With x' the stored activations
 //   sum_k (q - z) x = D - 1024 sum_k x' - z sum_k x,   D the mma's sum
-// is applied per 32-wide block, with the weight's scale, in fp32 (the magic's part is the C operand of the first
-// mma).  Activations are stored as fp16 after division by a power of two, one per token for x and one per
+// is applied per 32-wide block, with the weight's scale, in fp32.  Activations are stored as fp16 after division by a power of two, one per token for x and one per
 // 32-block and token for h, so their size does not matter: x loses nothing down to 2^-13 (bf16) or 2^-10
 // (fp16) of the token's largest and at most 2^-21 of the largest below that; h keeps 11 significant bits
 // between the kernels, 1/8 of a bf16 half step.
@@ -227,12 +226,11 @@ struct Ring {
   // Tile row of lane group g: G = 2 reads half pieces, which needs every other pair of rows in a phase.
   __device__ static int row_of(int g) { return G == 2 ? (g & 1) | (g & 2) << 1 | (g & 4) >> 1 : g; }
 
-  // Whether step s brings a window, in a run that began with step `start`.
-  __device__ static bool has_window(const MoeWeight& w, int s, int start) {
-    if (s == start) return true;
-    if (MODE == kOnePerBlock) return (s & 1) == 0;
-    if (MODE == kPowerOfTwo) return (s * 4 & ((8 << w.group_shift) - 1)) == 0;
-    return (s - start) % w.window == 0;
+  // The step after s (which brings a window) that brings the next one in its run.
+  __device__ static int next_window(const MoeWeight& w, int s) {
+    if (MODE == kOnePerBlock) return (s | 1) + 1;
+    if (MODE == kPowerOfTwo) return (s | ((2 << w.group_shift) - 1)) + 1;
+    return s + w.window;
   }
   // Place of step s's first group in the window that step w_s brought, for rows that are row_of(g) modulo 8.
   __device__ static int index_of(const MoeWeight& w, int s, int w_s, int g, int n_group) {
@@ -252,11 +250,12 @@ struct Ring {
     for (int i = 0; i < (ROWS * PIECES + 31) / 32; ++i) {
       const int row = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
       if (row >= ROWS) break;
-      const int64_t first = ((at + (int64_t)row * n_group) & ~7ll) + piece * 8;
-      const int left = (int)max((int64_t)0, min((int64_t)8, total - first)) * 2;
+      const int64_t first = ((at + row * n_group) & ~7ll) + piece * 8;
+      const int bytes = first + 8 <= total ? 16 : first < total ? (int)(total - first) * 2 : 0;
       const uint32_t dst = window + (row0 + row) * kWindowRow + piece * 16;
-      cp_async16(dst, w.scale + (left ? first : 0), left);
-      if (ASYM) cp_async16(dst + kZeros, w.zp + (left ? first : 0), left);
+      const int64_t from = bytes ? first : 0;
+      cp_async16(dst, w.scale + from, bytes);
+      if (ASYM) cp_async16(dst + kZeros, w.zp + from, bytes);
     }
   }
 };
@@ -335,12 +334,10 @@ __device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// d = {c0, c1, c0, c1} + a b
-__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
-                                         float c1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // What a block of two tokens brings besides its values: {m0, m1}, minus what the magic (and, for a symmetric
@@ -370,7 +367,6 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
   }
 #pragma unroll
   for (int j = 0; j < 4 / G; ++j) {
-    const int own = s * 4 + j * G + t / (4 / G);  // this lane's block of the set
     // its G words: 16-byte piece (block) of the row, word t mod 4 / G times G
     const int piece = ((j * G + t / (4 / G)) ^ (r0 >> 1 & 3)) * 16 + t % (4 / G) * (4 * G);
     uint32_t c[2 * R][G];
@@ -381,7 +377,8 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
       else if constexpr (G == 2) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(from);
       else c[i][0] = *reinterpret_cast<const uint32_t*>(from);
     }
-    const float2 m = *reinterpret_cast<const float2*>(sides.m + j * G * MS);
+    F2 m;
+    m.v = *reinterpret_cast<const unsigned long long*>(sides.m + j * G * MS);
     float d[R][4];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -390,7 +387,7 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
       for (int q = 0; q < R; ++q) {
         uint32_t a[2][4];
         a_operands(c[2 * q][i], c[2 * q + 1][i], a);
-        if (i == 0) mma_from(d[q], a[0], v.x, v.y, m.x, m.y);
+        if (i == 0) mma_first(d[q], a[0], v.x, v.y);
         else mma_add(d[q], a[0], v.x, v.y);
         mma_add(d[q], a[1], v.z, v.w);
       }
@@ -398,6 +395,9 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
     F2 f{}, s2{};
     if (SCALED) f.v = *reinterpret_cast<const unsigned long long*>(sides.f + j * G * MS);
     if (ASYM) s2.v = *reinterpret_cast<const unsigned long long*>(sides.s2 + j * G * MS);
+    // this lane's block of the set; past the row's last (whose products are zero) the last one's scale will do
+    int own = s * 4 + j * G + t / (4 / G);
+    if (MODE == kAny) own = min(own, n_blk - 1);
     const int group = MODE == kOnePerBlock ? 0 : (group_of(w, own) - group_of(w, s * 4)) * 2;
 #pragma unroll
     for (int q = 0; q < R; ++q)
@@ -409,15 +409,13 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
           if (ASYM) z = group_value<G>(zp[ASYM ? q : 0][h], j, t);
         } else {
           const uint8_t* from = at + (q * 16 + h * 8) * Rg::kWindowRow + group;
-          const bool in = MODE == kPowerOfTwo || own < n_blk;  // there every step is whole
-          scale = in ? half_bits(*reinterpret_cast<const uint16_t*>(from)) : 0.f;
-          if (ASYM) z = in ? half_bits(*reinterpret_cast<const uint16_t*>(from + Rg::kZeros)) : 0.f;
+          scale = half_bits(*reinterpret_cast<const uint16_t*>(from));
+          if (ASYM) z = half_bits(*reinterpret_cast<const uint16_t*>(from + Rg::kZeros));
         }
-        F2 v = pack(d[q][2 * h], d[q][2 * h + 1]);
-        if (ASYM) v = fma2(pack(-z, -z), s2, v);
-        F2 by = pack(scale, scale);
+        F2 by = pack(scale, scale), less = m;
         if (SCALED) by = mul2(by, f);
-        acc[q][h] = fma2(by, v, acc[q][h]);
+        if (ASYM) less = fma2(pack(-z, -z), s2, m);
+        acc[q][h] = fma2(by, pack(d[q][2 * h], d[q][2 * h + 1]), fma2(by, less, acc[q][h]));
       }
   }
 }
@@ -543,7 +541,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   // the warp's ring runs through its steps of all items
   const int code_ring = warp * stages * Rg::kCodes, window_ring = at.windows + warp * stages * Rg::kWindow;
   const int64_t total_groups = (int64_t)p.E * p.I * n_group;
-  int f_item = s_first < s_last ? first : last, f_s = s_first, f_stage = 0, f_window = 0, f_row = 0;
+  int f_item = s_first < s_last ? first : last, f_s = s_first, f_stage = 0, f_window = 0, f_row = 0, f_next = s_first;
   auto f_start = [&] {
     if (f_item < last) {
       const int u = f_item / tiles;
@@ -559,14 +557,19 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
         sm100::tma_load_2d(to, &maps.gate, &bars[f_stage], f_s * 64, f_row);
         sm100::tma_load_2d(to + 1024, &maps.up, &bars[f_stage], f_s * 64, f_row);
       }
-      if (Rg::has_window(p.gate, f_s, s_first)) {
+      if (f_s == f_next) {
+        f_next = Rg::next_window(p.gate, f_s);
         const uint32_t to = base + window_ring + f_window * Rg::kWindow;
         if (++f_window == stages) f_window = 0;
         const int64_t group = (int64_t)f_row * n_group + group_of(p.gate, f_s * 4);
         Rg::template fetch_window<16>(to, 0, p.gate, group, n_group, total_groups, lane);
         Rg::template fetch_window<16>(to, 16, p.up, group, n_group, total_groups, lane);
       }
-      if (++f_s == s_last) { f_s = s_first; ++f_item; f_start(); }
+      if (++f_s == s_last) {
+        f_s = f_next = s_first;
+        ++f_item;
+        f_start();
+      }
       if (++f_stage == stages) f_stage = 0;
     }
     cp_async_commit();
@@ -624,14 +627,15 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
       }
     }
     F2 acc[2][2] = {};
-    int w_s = 0;
+    int w_s = 0, w_next = s_first;
     for (int s = s_first; s < s_last; ++s) {
       ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
       cp_async_wait(stages - 1);
       __syncwarp();
-      if (Rg::has_window(p.gate, s, s_first)) {
+      if (s == w_next) {
         if (++window == stages) window = 0;
         w_s = s;
+        w_next = Rg::next_window(p.gate, s);
       }
       const int index = Rg::index_of(p.gate, s, w_s, g, n_group);
       const Sides here{sides.m + s * 32, nullptr, sides.s2 + s * 32};
@@ -774,40 +778,49 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
 
   const int64_t total_groups = (int64_t)p.E * p.H * n_group;
   const int first_u = first / n_steps, first_s = first - first_u * n_steps;
-  // a run is what the warp does of one unit
-  auto has_window = [&](int q, int s) { return Rg::has_window(p.down, s, q - s < first ? first_s : 0); };
-  int f_at = first, f_u = first_u, f_s = first_s, f_stage = 0, f_window = 0;
+  // a run of windows is what the warp does of one unit
+  int f_at = first, f_u = first_u, f_s = first_s, f_stage = 0, f_window = 0, f_next = first_s;
   auto fetch_weights = [&] {
     const int row0 = r.unit_expert[f_u] * p.H + j0;
     if (lane == 0) {
       sm100::mbar_arrive_expect_tx(&bars[f_stage], Rg::kCodes);
       sm100::tma_load_2d(dyn + code_ring + f_stage * Rg::kCodes, &map, &bars[f_stage], f_s * 64, row0);
     }
-    if (has_window(f_at, f_s)) {
+    if (f_s == f_next) {
+      f_next = Rg::next_window(p.down, f_s);
       Rg::template fetch_window<kDownRows>(base + rest_ring + f_window * at.stage, 0, p.down,
                                            (int64_t)row0 * n_group + group_of(p.down, f_s * 4), n_group, total_groups,
                                            lane);
       if (++f_window == stages) f_window = 0;
     }
   };
+  constexpr int kPieces = kRecord / 16, kParts = (NT / 2 * 4 * kPieces + 31) / 32;
+  int part_src[kParts];  // of this lane's 16-byte pieces of a step's records, from the unit's first of the step on
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const int c = i * 32 + lane, pair = c / (4 * kPieces);
+    part_src[i] = pair * n_blk * kRecord + (c - pair * 4 * kPieces) * 16;
+  }
   auto fetch_records = [&] {  // blocks 4 f_s .. + 4 of the unit's tokens; zeros past n_blk
-    constexpr int kPieces = kRecord / 16;
     const uint8_t* rec = p.h + ((int64_t)r.unit_slot[f_u] * n_blk + f_s * 4) * kRecord;
     const int pieces = (__popc(r.unit_mask[f_u]) + 1) / 2 * 4 * kPieces;
-    const uint32_t to = base + rest_ring + f_stage * at.stage + Rg::kWindow;
+    const uint32_t to = base + rest_ring + f_stage * at.stage + Rg::kWindow + lane * 16;
+    const int whole = (n_blk - f_s * 4) * kPieces;  // pieces of a pair that exist
 #pragma unroll
-    for (int c0 = 0; c0 < NT / 2 * 4 * kPieces; c0 += 32) {
-      const int c = c0 + lane, pair = c / (4 * kPieces), rest = c - pair * 4 * kPieces;
-      const bool valid = f_s * 4 + rest / kPieces < n_blk;
-      if (c < pieces)
-        cp_async16(to + c * 16, valid ? rec + (int64_t)pair * n_blk * kRecord + rest * 16 : p.h, valid ? 16 : 0);
+    for (int i = 0; i < kParts; ++i) {
+      const int c = i * 32 + lane;
+      const bool valid = MODE != kAny || c % (4 * kPieces) < whole;
+      if (c < pieces) cp_async16(to + i * 512, valid ? rec + part_src[i] : p.h, valid ? 16 : 0);
     }
   };
   auto advance = [&] {
     cp_async_commit();
     if (f_at < last) {
       ++f_at;
-      if (++f_s == n_steps) { f_s = 0; ++f_u; }
+      if (++f_s == n_steps) {
+        f_s = f_next = 0;
+        ++f_u;
+      }
       if (++f_stage == stages) f_stage = 0;
     }
   };
@@ -848,7 +861,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     if (f_at < last) fetch_records();
     advance();
   }
-  int c_u = first_u, c_s = first_s, stage = 0, window = -1, w_s = 0;
+  int c_u = first_u, c_s = first_s, stage = 0, window = -1, w_s = 0, w_next = first_s;
   uint32_t parity = 0;
   bool ok = true;
   for (int q = first; q < last; ++q) {
@@ -859,9 +872,10 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
     cp_async_wait(stages - 1);
     __syncwarp();
-    if (has_window(q, c_s)) {
+    if (c_s == w_next) {
       if (++window == stages) window = 0;
       w_s = c_s;
+      w_next = Rg::next_window(p.down, c_s);
     }
     const int index = Rg::index_of(p.down, c_s, w_s, g, n_group);
     const uint8_t* side = sides + stage * at.stage;
@@ -875,8 +889,14 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
       fetch_records();
     }
     advance();
-    if (++c_s == n_steps) { c_s = 0; ++c_u; }
-    if (++stage == stages) { stage = 0; parity ^= 1; }
+    if (++c_s == n_steps) {
+      c_s = w_next = 0;
+      ++c_u;
+    }
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
   }
   flush();
   asm volatile("cp.async.wait_all;" ::: "memory");
