@@ -78,7 +78,7 @@ struct MoeParams {
   uint64_t wait_ns;
 };
 
-// One 32-block of h of two tokens: 32 stored fp16 values of each (64 bytes), then {m0, m1, f0, f1, s2 of both}.
+// One 32-block of h of two tokens: 32 stored fp16 values of each (64 bytes), then {m0, m1, m0, m1, f0, f1, s2 of both}.
 constexpr int kRecord = 160;
 
 // ---- routing ---------------------------------------------------------------------------------
@@ -265,10 +265,10 @@ __device__ __forceinline__ float half_bits(uint32_t v) { return __half2float(__u
 // The value of this lane's block of set j among the four of a step.
 template <int G>
 __device__ __forceinline__ float group_value(const uint2& v, int j, int t) {
-  if (G == 4) return half_bits((t & 2 ? v.y : v.x) >> ((t & 1) * 16));
-  if (G == 2) return half_bits((j ? v.y : v.x) >> (t / 2 * 16));
-  const uint32_t w = j < 2 ? v.x : v.y;
-  return half_bits(j & 1 ? w >> 16 : w);
+  const uint32_t w = G == 4 ? (t & 2 ? v.y : v.x) : (G == 2 ? j : j / 2) ? v.y : v.x;
+  const __half2 pair = *reinterpret_cast<const __half2*>(&w);
+  if (G == 1) return j & 1 ? __high2float(pair) : __low2float(pair);
+  return half_bits(w >> (G == 4 ? (t & 1) * 16 : t / 2 * 16));
 }
 
 // Pair j of a word's codes, j and j + 4, as two fp16 values: 1024 + q (j even) or 1024 + 16 q (j odd).
@@ -302,56 +302,35 @@ __device__ __forceinline__ float power_below(float top) {
 // by 16).
 __device__ __forceinline__ void put_sides(float* m, float* s2, float even, float odd, bool asym) {
   const float sum = even + 16.f * odd, magic = -1024.f * (even + odd);
-  *m = asym ? magic : magic - 8.f * sum;
+  m[0] = m[2] = asym ? magic : magic - 8.f * sum;
   if (s2) *s2 = sum;
 }
 
-// Two floats in a register pair, for the packed fp32 instructions.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 pack(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack(const F2& x, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
-}
-__device__ __forceinline__ F2 mul2(const F2& a, const F2& b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(const F2& a, const F2& b, const F2& c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 // mma.sync.m16n8k16 fp16; a plain (not volatile) asm, so that the compiler may interleave the tiles
 __device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                         const float4& c) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 
-// What a block of two tokens brings besides its values: {m0, m1}, minus what the magic (and, for a symmetric
-// weight, z = 8) adds; their powers of two and their sums, each where a kernel has them per block.
+// What a block of two tokens brings besides its values: {m0, m1, m0, m1}, minus what the magic (and, for a
+// symmetric weight, z = 8) adds, as the first mma's C operand; their powers of two and their sums.
 struct Sides {
   const uint8_t *m, *f, *s2;
 };
 
-// Adds one step to acc[tile][row_of(g), + 8] (two tokens each).  `codes` and `window` are the ring's; `index` the place
+// Adds one step to acc[tile] (rows row_of(g) and + 8 of two tokens, as the mma has them).  `codes` and `window` are the ring's; `index` the place
 // of the step's first group in this lane's row of the window; `operand` this lane's part of the first set in B
 // order, BLOCK bytes from block to block (a lane off the diagonal: zeros); `sides` belong to its two tokens and its
-// block of the first set, MS bytes from block to block.
-template <int G, int R, bool ASYM, int MODE, bool SCALED, int BLOCK, int MS>
-__device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, const uint8_t* window, int index,
+// block of the first set, MS and FS bytes from block to block.
+template <int G, int R, bool ASYM, int MODE, bool SCALED, int BLOCK, int MS, int FS>
+__device__ __forceinline__ void add_step(float (&acc)[R][4], const uint8_t* codes, const uint8_t* window, int index,
                                          const uint8_t* operand, const Sides& sides, int g, int t, int s, int n_blk,
                                          const MoeWeight& w) {
   using Rg = Ring<G, R, ASYM, MODE>;
@@ -377,8 +356,7 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
       else if constexpr (G == 2) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(from);
       else c[i][0] = *reinterpret_cast<const uint32_t*>(from);
     }
-    F2 m;
-    m.v = *reinterpret_cast<const unsigned long long*>(sides.m + j * G * MS);
+    const float4 m = *reinterpret_cast<const float4*>(sides.m + j * G * MS);
     float d[R][4];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -387,14 +365,14 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
       for (int q = 0; q < R; ++q) {
         uint32_t a[2][4];
         a_operands(c[2 * q][i], c[2 * q + 1][i], a);
-        if (i == 0) mma_first(d[q], a[0], v.x, v.y);
+        if (i == 0) mma_from(d[q], a[0], v.x, v.y, m);
         else mma_add(d[q], a[0], v.x, v.y);
         mma_add(d[q], a[1], v.z, v.w);
       }
     }
-    F2 f{}, s2{};
-    if (SCALED) f.v = *reinterpret_cast<const unsigned long long*>(sides.f + j * G * MS);
-    if (ASYM) s2.v = *reinterpret_cast<const unsigned long long*>(sides.s2 + j * G * MS);
+    float2 f = make_float2(1.f, 1.f), s2 = make_float2(0.f, 0.f);
+    if (SCALED) f = *reinterpret_cast<const float2*>(sides.f + j * G * FS);
+    if (ASYM) s2 = *reinterpret_cast<const float2*>(sides.s2 + j * G * FS);
     // this lane's block of the set; past the row's last (whose products are zero) the last one's scale will do
     int own = s * 4 + j * G + t / (4 / G);
     if (MODE == kAny) own = min(own, n_blk - 1);
@@ -412,10 +390,13 @@ __device__ __forceinline__ void add_step(F2 (&acc)[R][2], const uint8_t* codes, 
           scale = half_bits(*reinterpret_cast<const uint16_t*>(from));
           if (ASYM) z = half_bits(*reinterpret_cast<const uint16_t*>(from + Rg::kZeros));
         }
-        F2 by = pack(scale, scale), less = m;
-        if (SCALED) by = mul2(by, f);
-        if (ASYM) less = fma2(pack(-z, -z), s2, m);
-        acc[q][h] = fma2(by, pack(d[q][2 * h], d[q][2 * h + 1]), fma2(by, less, acc[q][h]));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float fk = k ? f.y : f.x, sk = k ? s2.y : s2.x;
+          float v = d[q][2 * h + k];
+          if (ASYM) v = fmaf(-z, sk, v);
+          acc[q][2 * h + k] = fmaf(SCALED ? scale * fk : scale, v, acc[q][2 * h + k]);
+        }
       }
   }
 }
@@ -442,7 +423,8 @@ constexpr int kUpSlices = 8;
 constexpr int kMaxStages = 4;    // of a ring
 
 // Shared memory of kernel 1 behind the routing: the warps' rings (codes, windows), tokens [NT][4 * steps] blocks of
-// 64 bytes (neighbouring rows in the other half of the banks), their m and s2 [NT / 2][blocks], the partial
+// 64 bytes (neighbouring rows in the other half of the banks), their m [NT / 2][blocks + 1] (pairs in different
+// banks) and s2 [NT / 2][blocks], the partial
 // products, 256 bytes of zeros, barriers.
 struct UpLayout {
   int windows, x, row, m, s2, red, zeros, bars, bytes;
@@ -452,7 +434,7 @@ struct UpLayout {
     x = windows + kUpWarps * stages * window_bytes;
     row = blocks * 64 + 64;
     m = x + row * nt;
-    s2 = m + nt / 2 * blocks * 8;
+    s2 = m + nt / 2 * (blocks + 1) * 16;
     red = s2 + (asym ? nt / 2 * blocks * 8 : 0);
     zeros = red + kUpSlices * 2 * kUpRows * nt * 4;
     bars = zeros + 256;
@@ -535,8 +517,9 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   const bool diag = g / NT == lane_blk;  // it holds the nonzero part of column g
   const uint8_t* operand = dyn + (diag ? at.x + (g % NT) * at.row + lane_blk * 64 + t % (4 / G) * G * 16 : at.zeros);
   const int operand_step = diag ? 256 : 0;
-  const int pair_blk = (t % (4 / G) * blocks + lane_blk) * 8;
-  const Sides sides{dyn + at.m + pair_blk, nullptr, dyn + at.s2 + pair_blk};
+  const int pair = t % (4 / G);
+  const Sides sides{dyn + at.m + (pair * (blocks + 1) + lane_blk) * 16, nullptr,
+                    dyn + at.s2 + (pair * blocks + lane_blk) * 8};
 
   // the warp's ring runs through its steps of all items
   const int code_ring = warp * stages * Rg::kCodes, window_ring = at.windows + warp * stages * Rg::kWindow;
@@ -611,9 +594,8 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
               continue;
             }
             uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
-            const int pb = (i / 2 * blocks + (j >> 2)) * 2 + (i & 1);
-            float* to_m = reinterpret_cast<float*>(dyn + at.m) + pb;
-            float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + pb : nullptr;
+            float* to_m = reinterpret_cast<float*>(dyn + at.m) + (i / 2 * (blocks + 1) + (j >> 2)) * 4 + (i & 1);
+            float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + (i / 2 * blocks + (j >> 2)) * 2 + (i & 1) : nullptr;
             const bool write = j < blocks * 4;
             if (p.dtype == NPB_BF16) store_operand<__nv_bfloat16>(raw, 1.f / f, to, to_m, to_s2, write, ASYM);
             else store_operand<__half>(raw, 1.f / f, to, to_m, to_s2, write, ASYM);
@@ -626,7 +608,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
         __syncthreads();
       }
     }
-    F2 acc[2][2] = {};
+    float acc[2][4] = {};
     int w_s = 0, w_next = s_first;
     for (int s = s_first; s < s_last; ++s) {
       ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
@@ -638,8 +620,8 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
         w_next = Rg::next_window(p.gate, s);
       }
       const int index = Rg::index_of(p.gate, s, w_s, g, n_group);
-      const Sides here{sides.m + s * 32, nullptr, sides.s2 + s * 32};
-      add_step<G, 2, ASYM, MODE, false, 64, 8>(acc, dyn + code_ring + stage * Rg::kCodes,
+      const Sides here{sides.m + s * 64, nullptr, sides.s2 + s * 32};
+      add_step<G, 2, ASYM, MODE, false, 64, 16, 8>(acc, dyn + code_ring + stage * Rg::kCodes,
                                                dyn + window_ring + window * Rg::kWindow, index, operand + s * operand_step, here, g, t, s, n_blk, p.gate);
       __syncwarp();
       fetch();
@@ -652,11 +634,9 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
     for (int w = 0; w < 2; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v[2];
-        unpack(acc[w][h], v[0], v[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float q = block_sum<G>(v[c]);
+          const float q = block_sum<G>(acc[w][2 * h + c]);
           if (t < 4 / G) part[(w * NT + 2 * t + c) * kUpRows + mt * 16 + Rg::row_of(g) + h * 8] = q;
         }
       }
@@ -689,8 +669,8 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
       reinterpret_cast<__half*>(rec)[(warp & 1) * 32 + (lane & 24) + (lane & 3) * 2 + ((lane >> 2) & 1)] = v;
       if (lane == 0) {
         float* to = reinterpret_cast<float*>(rec + 128) + (warp & 1);
-        put_sides(to, to + 4, even, odd, p.down.zp != nullptr);
-        to[2] = f;
+        put_sides(to, to + 6, even, odd, p.down.zp != nullptr);
+        to[4] = f;
       }
     }
   }
@@ -825,7 +805,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     }
   };
 
-  F2 acc[kDownTiles][2] = {};
+  float acc[kDownTiles][4] = {};
   int unit = -1;
   auto flush = [&] {
     uint32_t m = unit >= 0 ? r.unit_mask[unit] : 0u;
@@ -835,14 +815,12 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     for (int w = 0; w < kDownTiles; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v[2];
-        unpack(acc[w][h], v[0], v[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float q = block_sum<G>(v[c]);
+          const float q = block_sum<G>(acc[w][2 * h + c]);
           if (t < 4 / G && token[c] >= 0) sums[token[c] * kDownRows + w * 16 + h * 8 + Rg::row_of(g)] += q;
+          acc[w][2 * h + c] = 0.f;
         }
-        acc[w][h] = F2{0ull};
       }
     __syncwarp();
   };
@@ -879,9 +857,9 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     }
     const int index = Rg::index_of(p.down, c_s, w_s, g, n_group);
     const uint8_t* side = sides + stage * at.stage;
-    add_step<G, kDownTiles, ASYM, MODE, true, kRecord, kRecord>(acc, dyn + code_ring + stage * Rg::kCodes,
+    add_step<G, kDownTiles, ASYM, MODE, true, kRecord, kRecord, kRecord>(acc, dyn + code_ring + stage * Rg::kCodes,
                                                                 dyn + rest_ring + window * at.stage, index, operand + stage * operand_stage,
-                                                                Sides{side, side + 8, side + 16}, g, t, c_s, n_blk,
+                                                                Sides{side, side + 16, side + 24}, g, t, c_s, n_blk,
                                                                 p.down);
     __syncwarp();
     if (f_at < last) {
