@@ -36,7 +36,7 @@ SOURCES = [
     "gemm_tcgen05.cu",
     "vq_gemm_fused.cu",
     "static_scratch.cu",
-    "allgather_push.cu", "rms_norm.cu", "vq_gemv_mma.cu", "embedding.cu", "vq_entropy.cu", "vq_decode_copy.cu", "q_gemm_staged.cu", "vq_lut.cu", "token_logprobs.cu", "q_moe.cu",
+    "allgather_push.cu", "rms_norm.cu", "vq_gemv_mma.cu", "embedding.cu", "vq_entropy.cu", "vq_decode_copy.cu", "q_gemm_staged.cu", "vq_lut.cu", "token_logprobs.cu", "q_moe.cu", "gemm_skinny.cu",
 ]
 
 NVCC_FLAGS = [

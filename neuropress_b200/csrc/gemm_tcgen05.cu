@@ -810,6 +810,10 @@ int gemm(const void* x, const void* w, const float* bias, void* y, int64_t M, in
   return gemm_impl(x, w, bias, y, M, N, K, dtype, nullptr, st);
 }
 
+// gemm_skinny.cu
+int gemm_skinny(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, int64_t M,
+                int64_t N, int64_t K, int dtype, cudaStream_t st);
+
 // y = T(act(x W^T + bias) + residual): the dense GEMM with the rest of a decoder block's step in its epilogue.
 int gemm_epilogue(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, int64_t M,
                   int64_t N, int64_t K, int dtype, cudaStream_t st) {
@@ -819,6 +823,8 @@ int gemm_epilogue(const void* x, const void* w, const float* bias, int act, cons
   if (w == nullptr) return NPB_ERR_INVALID_ARG;
   if (!aligned_to(w, 16) || !aligned_to(y, 2) || !aligned_to(residual, 2) || !aligned_to(bias, 4))
     return NPB_ERR_ALIGNMENT;
+  static const int skinny_rows = [] { const char* e = getenv("NPB_SKINNY"); return e ? atoi(e) : 256; }();
+  if (M <= skinny_rows) return gemm_skinny(x, w, bias, act, residual, y, M, N, K, dtype, st);
   GemmParams p{};
   p.bias = bias;
   p.y = y;
@@ -897,6 +903,7 @@ int vq_gemm_fused_device_status(int* host_out);  // vq_gemm_fused.cu keeps its o
 int q_gemv_ring_device_status(int* host_out);    // and so does q_gemv_ring.cu
 int vq_decode_copy_device_status(int* host_out); // and vq_decode_copy.cu
 int q_moe_device_status(int* host_out);          // and q_moe.cu
+int gemm_skinny_device_status(int* host_out);    // and gemm_skinny.cu
 
 int gemm_device_status(int* host_out) {
   int v = 0;
@@ -920,6 +927,9 @@ int gemm_device_status(int* host_out) {
   int vm = 0;
   if (int rc = q_moe_device_status(&vm)) return rc;
   if (v == 0 && vm != 0) v = 50 + vm;
+  int vk = 0;
+  if (int rc = gemm_skinny_device_status(&vk)) return rc;
+  if (v == 0 && vk != 0) v = 60 + vk;
   if (host_out) *host_out = v;
   return v == 0 ? NPB_OK : NPB_ERR_DEVICE_TIMEOUT;
 }
