@@ -7,8 +7,12 @@
 // x][128] meet in shared memory and each CTA finishes an equal share of them, reading its peers' over DSMEM in rank
 // order -- no workspace, no atomics, the same bits every time.
 //
-// CTA: warp 0 TMA producer (stages of 128 of k: two 64-wide boxes of W and of x, 128-byte swizzle), warp 1 TMEM owner
-// and tcgen05.mma issuer, warps 2-9 move the accumulator (TMEM lane = output, column = row of x) to shared memory or,
+// With more than 128 rows and many tiles two CTAs pair up on 256 outputs (cta_group::2): each loads its 128 rows of W
+// and half of the rows of x, so x crosses from L2 once per 256 outputs; with that many rows the traffic into the SMs is
+// what bounds the kernel (6.5-7.8 TB/s were measured without pairs).
+//
+// CTA: warp 0 TMA producer (stages of 64 or 128 of k: 64-wide boxes of W and of x, 128-byte swizzle), warp 1 TMEM owner
+// and tcgen05.mma issuer; then all eight warps move the accumulator (TMEM lane = output, column = row of x) to shared memory or,
 // unsplit, straight through the epilogue; lanes are consecutive outputs, so stores and residual loads are coalesced,
 // and the residual is on its way before the sums are there.  Up to two CTAs share an SM.  Every wait is bounded (npb_set_wait_limit_ns); on give-up the kernel records it, lets
 // its copies land, frees its TMEM and returns.
@@ -31,9 +35,8 @@ namespace {
 using namespace sm100;
 
 constexpr int BN = 128;             // outputs per tile
-constexpr int BK = 128;             // of k per stage, as two halves of 64 (one swizzle row each)
-constexpr int kThreads = 320;
-constexpr int kWHalf = BN * 64 * 2; // 16 KiB
+constexpr int kThreads = 256;  // eight warps: two CTAs fit an SM's register banks (ten warps of 96 registers do not)
+constexpr int kWBox = BN * 64 * 2;  // 16 KiB: 64 of k (one swizzle row) of the tile's rows of W
 constexpr int kMaxStages = 8;
 constexpr int kHead = 1024;         // barriers
 
@@ -43,7 +46,9 @@ struct SkinnyParams {
   void* y;
   int M, N, act;
   int rows;       // of x per tile: multiple of 16, at most 256
-  int stages, k_blocks, split;
+  int boxes;      // of 64 of k per stage: 1 or 2
+  int stages, k_stages, split;
+  int part_rows;  // rows of x whose partial sums fit the ring
   uint64_t wait_ns;
 };
 
@@ -52,7 +57,7 @@ __device__ __forceinline__ float residual_at(const SkinnyParams& p, int m, int n
   return to_f32(static_cast<const T*>(p.residual)[(int64_t)m * p.N + n]);
 }
 
-template <typename T>
+template <typename T, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 2)
 gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const SkinnyParams p) {
@@ -64,12 +69,14 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* ring = smem + kHead;
-  const int x_half = p.rows * 128, stage_bytes = 2 * kWHalf + 2 * x_half;
+  constexpr int CG = PAIR ? 2 : 1;
+  const int x_box = p.rows / CG * 128, stage_bytes = p.boxes * (kWBox + x_box);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = p.split > 1 ? (int)cluster_ctarank() : 0;
-  const int n0 = blockIdx.x / p.split * BN, m0 = blockIdx.y * p.rows;
-  const int kb0 = (int)((int64_t)p.k_blocks * rank / p.split), kb1 = (int)((int64_t)p.k_blocks * (rank + 1) / p.split);
+  const int cta = PAIR || p.split > 1 ? (int)cluster_ctarank() : 0;
+  const int rank = cta / CG, side = cta % CG;  // share of K; half of the pair
+  const int n0 = (blockIdx.x / (CG * p.split) * CG + side) * BN, m0 = blockIdx.y * p.rows;
+  const int kb0 = (int)((int64_t)p.k_stages * rank / p.split), kb1 = (int)((int64_t)p.k_stages * (rank + 1) / p.split);
   const uint32_t tmem_cols = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : p.rows <= 128 ? 128 : 256;
 
   if (tid == 0) {
@@ -84,11 +91,21 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tma_prefetch_desc(&map_x);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, tmem_cols);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(tmem_slot, tmem_cols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, tmem_cols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) {
+    __syncwarp();
+    cluster_sync_all();  // the peer's barriers exist before anything is sent to them
+  } else {
+    __syncthreads();
+  }
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
@@ -102,17 +119,26 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           break;
         }
         uint8_t* st = ring + (size_t)s * stage_bytes;
-        mbar_arrive_expect_tx(&full[s], (uint32_t)stage_bytes);
-        tma_load_2d(st, &map_w, &full[s], kb * BK, n0);
-        tma_load_2d(st + kWHalf, &map_w, &full[s], kb * BK + 64, n0);
-        tma_load_2d(st + 2 * kWHalf, &map_x, &full[s], kb * BK, m0);
-        tma_load_2d(st + 2 * kWHalf + x_half, &map_x, &full[s], kb * BK + 64, m0);
+        // all bytes of a pair's stage are credited to its even CTA's barrier
+        if (side == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * stage_bytes));
+        for (int h = 0; h < p.boxes; ++h) {
+          const int k = (kb * p.boxes + h) * 64;
+          if (PAIR) {
+            const uint32_t bar = map_to_cta(smem_u32(&full[s]), cta & ~1);
+            tma_load_2d_pair(st + h * kWBox, &map_w, bar, k, n0);
+            tma_load_2d_pair(st + p.boxes * kWBox + h * x_box, &map_x, bar, k, m0 + side * (p.rows / 2));
+          } else {
+            tma_load_2d(st + h * kWBox, &map_w, &full[s], k, n0);
+            tma_load_2d(st + p.boxes * kWBox + h * x_box, &map_x, &full[s], k, m0);
+          }
+        }
         if (++s == p.stages) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, BN, p.rows);
+    if (lane == 0 && side == 0) {
+      const uint32_t idesc = umma_idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, CG * BN, p.rows);
+      const uint32_t both = 3u << (cta & ~1);
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -124,116 +150,137 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         tc_fence_after();
         const uint32_t st = smem_u32(ring + (size_t)s * stage_bytes);
+        for (int h = 0; h < p.boxes; ++h) {
+          const uint64_t a = umma_desc_sw128(st + h * kWBox), b = umma_desc_sw128(st + p.boxes * kWBox + h * x_box);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint64_t a = umma_desc_sw128(st + h * kWHalf), b = umma_desc_sw128(st + 2 * kWHalf + h * x_half);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16(tmem, a + 2 * k, b + 2 * k, idesc, (kb > kb0 || h > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t more = (kb > kb0 || h > 0 || k > 0) ? 1u : 0u;
+            if (PAIR) umma_f16_pair(tmem, a + 2 * k, b + 2 * k, idesc, more);
+            else umma_f16(tmem, a + 2 * k, b + 2 * k, idesc, more);
+          }
         }
-        umma_commit(&empty[s]);
+        if (PAIR) umma_commit_pair(&empty[s], both);
+        else umma_commit(&empty[s]);
         if (++s == p.stages) { s = 0; ph ^= 1; }
       }
-      if (ok) umma_commit(done);
+      if (ok) {
+        if (PAIR) umma_commit_pair(done, both);
+        else umma_commit(done);
+      }
     }
-  } else {
-    // 16 rows of x at a time: two warps share the 32 outputs of a TMEM quadrant
-    const int quad = warp & 3, n = quad * 32 + lane, c0 = warp < 6 ? 0 : 16;  // TMEM lane = output of the tile
-    const int rows = min(p.rows, p.M - m0);
-    const bool in = n0 + n < p.N, adds = p.split == 1 && p.residual != nullptr && in;
-    const float bias = p.split == 1 && p.bias && in ? __ldg(p.bias + n0 + n) : 0.f;
+  }
+  __syncwarp();
+  // Epilogue, 16 rows of x at a time: two warps share the 32 outputs of a TMEM quadrant.
+  const int quad = warp & 3, lane_n = quad * 32 + lane, c0 = warp < 4 ? 0 : 16;  // TMEM lane = output of the tile
+  const int rows = min(p.rows, p.M - m0);
+  const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16);
+  if (p.split == 1) {
+    const bool in = n0 + lane_n < p.N, adds = p.residual != nullptr && in;
+    const float bias = p.bias && in ? __ldg(p.bias + n0 + lane_n) : 0.f;
     float r[16];
     auto load_residual = [&](int c) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) r[i] = adds && c + i < rows ? residual_at<T>(p, m0 + c + i, n0 + n) : 0.f;
+      for (int i = 0; i < 16; ++i) r[i] = adds && c + i < rows ? residual_at<T>(p, m0 + c + i, n0 + lane_n) : 0.f;
     };
     load_residual(c0);
-    const bool got = mbar_wait_bounded(done, 0, abort_flag, p.wait_ns, 64u);
-    if (__all_sync(0xffffffffu, got)) {
+    if (__all_sync(0xffffffffu, mbar_wait_bounded(done, 0, abort_flag, p.wait_ns, 64u))) {
       tc_fence_after();
-      float* part = reinterpret_cast<float*>(ring);   // every stage has been read
       for (int c = c0; c < rows; c += 32) {
         uint32_t v[16];
-        tmem_ld_32x32_x16(tmem + ((uint32_t)(quad * 32) << 16) + c, v);
+        tmem_ld_32x32_x16(acc + c, v);
         tmem_ld_wait();
-        if (p.split > 1) {
+        T* y = static_cast<T*>(p.y) + (int64_t)(m0 + c) * p.N + n0 + lane_n;
+        float o[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[(c + i) * BN + n] = __uint_as_float(v[i]);
-        } else {
-          T* y = static_cast<T*>(p.y) + (int64_t)(m0 + c) * p.N + n0 + n;
-          float o[16];
+        for (int i = 0; i < 16; ++i) o[i] = activate(__uint_as_float(v[i]) + bias, p.act) + r[i];
+        load_residual(c + 32);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = activate(__uint_as_float(v[i]) + bias, p.act) + r[i];
-          load_residual(c + 32);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (in && c + i < rows) y[(int64_t)i * p.N] = from_f32<T>(o[i]);
-        }
+        for (int i = 0; i < 16; ++i)
+          if (in && c + i < rows) y[(int64_t)i * p.N] = from_f32<T>(o[i]);
       }
     } else {
       atomicExch(&g_skinny_status, 3);
     }
     tc_fence_before();
-  }
-  __syncwarp();
-  if (p.split > 1) {
-    // each CTA of the cluster finishes an equal share of the tile, four outputs of a row of x at a time, adding the
-    // partial sums in rank order
-    const int rows = min(p.rows, p.M - m0), total = rows * (BN / 4);
-    const int last = (int)((int64_t)total * (rank + 1) / p.split);
-    int i = (int)((int64_t)total * rank / p.split) + tid;
+  } else {
+    // The partial sums go to the ring (every stage has been read), as many rows of x as it holds; each CTA of the
+    // cluster finishes an equal share of them, four outputs of a row at a time, adding them in rank order.
+    const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(done, 0, abort_flag, p.wait_ns, 64u));
+    if (!got) atomicExch(&g_skinny_status, 3);
+    tc_fence_after();
     struct alignas(8) Four { T e[4]; };
     const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 &&
                       (reinterpret_cast<uintptr_t>(p.residual) & 7) == 0;
-    float r[4], bias[4];
-    auto load_rest = [&](int u) {
-      const int n = n0 + u % (BN / 4) * 4, m = m0 + u / (BN / 4);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        bias[k] = p.bias && u < last && n + k < p.N ? __ldg(p.bias + n + k) : 0.f;
-        r[k] = 0.f;
+    const uint32_t part = smem_u32(ring);
+    for (int first = 0; first < rows; first += p.part_rows) {
+      const int here = min(p.part_rows, rows - first), total = here * (BN / 4);
+      if (first > 0) {
+        __syncwarp();
+        cluster_sync_all();  // the rows before are finished
       }
-      if (p.residual && u < last) {
-        if (wide && n < p.N) {
-          const Four f = *reinterpret_cast<const Four*>(static_cast<const T*>(p.residual) + (int64_t)m * p.N + n);
+      if (got) {
+        float* to = reinterpret_cast<float*>(ring);
+        for (int c = c0; c < here; c += 32) {
+          uint32_t v[16];
+          tmem_ld_32x32_x16(acc + first + c, v);
+          tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) r[k] = to_f32(f.e[k]);
+          for (int i = 0; i < 16; ++i) to[(c + i) * BN + lane_n] = __uint_as_float(v[i]);
+        }
+      }
+      const int last = (int)((int64_t)total * (rank + 1) / p.split);
+      int i = (int)((int64_t)total * rank / p.split) + tid;
+      float r[4], bias[4];
+      auto load_rest = [&](int u) {
+        const int n = n0 + u % (BN / 4) * 4, m = m0 + first + u / (BN / 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          bias[k] = p.bias && u < last && n + k < p.N ? __ldg(p.bias + n + k) : 0.f;
+          r[k] = 0.f;
+        }
+        if (p.residual && u < last) {
+          if (wide && n < p.N) {
+            const Four f = *reinterpret_cast<const Four*>(static_cast<const T*>(p.residual) + (int64_t)m * p.N + n);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[k] = to_f32(f.e[k]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n + k < p.N) r[k] = residual_at<T>(p, m, n + k);
+          }
+        }
+      };
+      load_rest(i);
+      __syncwarp();
+      cluster_sync_all();
+      for (; i < last; i += kThreads) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int c = 0; c < p.split; ++c) {
+          float4 q;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w)
+                       : "r"(map_to_cta(part + i * 16, c * CG + side))
+                       : "memory");
+          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+        }
+        const int n = n0 + i % (BN / 4) * 4, m = m0 + first + i / (BN / 4);
+        T* y = static_cast<T*>(p.y) + (int64_t)m * p.N + n;
+        Four f;
+        const float sum[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.e[k] = from_f32<T>(activate(sum[k] + bias[k], p.act) + r[k]);
+        if (wide && n < p.N) {
+          *reinterpret_cast<Four*>(y) = f;
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (n + k < p.N) r[k] = residual_at<T>(p, m, n + k);
+            if (n + k < p.N) y[k] = f.e[k];
         }
+        load_rest(i + kThreads);
       }
-    };
-    load_rest(i);
-    cluster_sync_all();
-    const uint32_t part = smem_u32(ring);
-    for (; i < last; i += kThreads) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int c = 0; c < p.split; ++c) {
-        float4 q;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w)
-                     : "r"(map_to_cta(part + i * 16, c))
-                     : "memory");
-        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-      }
-      const int n = n0 + i % (BN / 4) * 4, m = m0 + i / (BN / 4);
-      T* y = static_cast<T*>(p.y) + (int64_t)m * p.N + n;
-      Four f;
-      const float sum[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) f.e[k] = from_f32<T>(activate(sum[k] + bias[k], p.act) + r[k]);
-      if (wide && n < p.N) {
-        *reinterpret_cast<Four*>(y) = f;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (n + k < p.N) y[k] = f.e[k];
-      }
-      load_rest(i + kThreads);
     }
+    tc_fence_before();
     __syncwarp();
     cluster_sync_all();  // nobody leaves while its sums are read
   }
@@ -241,14 +288,72 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
-  __syncthreads();
+  if (PAIR) {
+    __syncwarp();
+    cluster_sync_all();  // nothing of the peer is touched after it left
+  } else {
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, tmem_cols);
+    if (PAIR) tmem_dealloc_pair(tmem, tmem_cols);
+    else tmem_dealloc(tmem, tmem_cols);
   }
 }
 
+template <typename T, bool PAIR>
+int launch_skinny(const cudaLaunchConfig_t& cfg, const CUtensorMap& map_w, const CUtensorMap& map_x,
+                  const SkinnyParams& p) {
+  auto kern = gemm_skinny_kernel<T, PAIR>;
+  int resident = 0;
+  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kThreads, cfg.dynamicSmemBytes, &resident)) return rc;
+  if (resident < 1) return NPB_ERR_TOO_LARGE;
+  NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, map_w, map_x, p));
+  NPB_LAUNCH_CHECK();
+  return NPB_OK;
+}
+
 }  // namespace
+
+// CTAs of this kernel that run at once, one to an SM, in clusters of a size (a GPC's SMs do not divide evenly: 132 in
+// clusters of four, 120 in clusters of eight on a B200).
+int resident_ctas(int cluster, int* ctas) {
+  static int cached[64][4] = {};
+  int dev = 0, slot = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
+  NPB_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return NPB_ERR_CUDA;
+  if (cached[dev][slot] == 0) {
+    auto kern = gemm_skinny_kernel<__half, false>;
+    int per_sm = 0;
+    const int smem = max_dynamic_smem() / 2 + 2048;
+    if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kThreads, smem, &per_sm)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(sm_count() / cluster * cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    NPB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+    cached[dev][slot] = n > 0 ? n * cluster : cluster;
+  }
+  *ctas = cached[dev][slot];
+  return NPB_OK;
+}
+
+// Whether this form is the faster one: up to 256 rows for every N, and above where the dense kernel's tiles leave SMs
+// idle -- up to 64 tiles in all (512 x 2048 x 8192: 29 / 50 us; 1024 x 8192 x 8192 with 256: 182 / 126 us), or one wave
+// of them with fewer rows each (400 x 8192 x 8192: 87 / 92 us; 512: 95 / 84 us).
+bool gemm_skinny_takes(int64_t M, int64_t N) {
+  const int64_t row_tiles = (M + 255) / 256, all = row_tiles * ((N + BN - 1) / BN);
+  const int64_t rows = row_tiles ? (M + row_tiles - 1) / row_tiles : 0;
+  return row_tiles <= 1 || all <= 64 || (all <= sm_count() && rows <= 208);
+}
 
 // Tiles of at most 256 rows of x; W is read once per tile of rows.
 int gemm_skinny(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, int64_t M,
@@ -259,48 +364,56 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   p.y = y;
   p.M = (int)M; p.N = (int)N; p.act = act;
   const int row_tiles = (int)((M + 255) / 256);
-  p.rows = (int)(((M + row_tiles - 1) / row_tiles + 15) / 16 * 16);
-  p.k_blocks = (int)((K + BK - 1) / BK);
+  const int rows = (int)((M + row_tiles - 1) / row_tiles);
+  // Pairs where more than 128 rows meet so many tiles that a split in two will do (201 rows, 14336 x 4096: 49 us against
+  // 59 us without; 128 rows: 38 / 36 us).  Split further they need clusters of eight, two CTAs to an SM, on half of the
+  // SMs (201 rows, 4096 x 14336: 53 / 40 us).
+  const bool pair = rows > 128 && (N + BN - 1) / BN >= 96;
+  const int cg = pair ? 2 : 1, step = 16 * cg;
+  p.rows = (rows + step - 1) / step * step;
   p.wait_ns = wait_limit_ns();
-  const int stage_bytes = 2 * kWHalf + 2 * p.rows * 128;
-  // two CTAs on an SM where three stages of each fit
+  const int box_bytes = kWBox + p.rows / cg * 128;  // of W and x, 64 of k
+  // two CTAs on an SM where three boxes of each fit
   const int half = max_dynamic_smem() / 2 - 1024 - 2048, whole = max_dynamic_smem() - 2048;
-  const int per_sm = (half - kHead) / stage_bytes >= 3 ? 2 : 1;
-  p.stages = ((per_sm == 2 ? half : whole) - kHead) / stage_bytes;
-  if (p.stages > kMaxStages) p.stages = kMaxStages;
-  const int64_t tiles = (N + BN - 1) / BN, slots = (int64_t)sm_count() * per_sm;
+  const int per_sm = (half - kHead) / box_bytes >= 3 ? 2 : 1, room = (per_sm == 2 ? half : whole) - kHead;
+  p.boxes = room / box_bytes >= 6 ? 2 : 1;
+  const int stage_bytes = p.boxes * box_bytes;
+  p.stages = room / stage_bytes < kMaxStages ? room / stage_bytes : kMaxStages;
+  p.k_stages = (int)((K + p.boxes * 64 - 1) / (p.boxes * 64));
+  const int64_t tiles = (N + cg * BN - 1) / (cg * BN) * cg;
   p.split = 1;
-  while (p.split < 8 && tiles * row_tiles * p.split * 2 <= slots && p.k_blocks >= p.split * 4) p.split *= 2;
-  const int parts = p.rows * BN * 4;
-  int ring = p.stages * stage_bytes;
-  if (ring < parts) ring = parts;
-  const int smem = 1024 + kHead + ring;
+  while (p.split * cg < (pair ? 4 : 8) && p.k_stages >= p.split * 4) {
+    int room_for = 0;  // CTAs that run at once, one to an SM, in clusters of twice the size
+    if (int rc = resident_ctas(p.split * cg * 2, &room_for)) return rc;
+    // a tenth more than run at once is better than half as many where two share an SM (1 row, 4096 x 14336: 256 CTAs
+    // 24 us, 128 CTAs 25 us), and worse where they do not (256 rows, 2048 x 2048: 128 CTAs 24 us, 64 CTAs 19 us)
+    const int64_t most = per_sm == 2 ? room_for * 2 * 11 / 10 : room_for;
+    if (tiles * row_tiles * p.split * 2 > most) break;
+    p.split *= 2;
+  }
+  const int ring = p.stages * stage_bytes;
+  p.part_rows = ring / (BN * 4) / 32 * 32;
   const bool bf16 = dtype == NPB_BF16;
-  const void* kern = bf16 ? reinterpret_cast<const void*>(gemm_skinny_kernel<__nv_bfloat16>)
-                          : reinterpret_cast<const void*>(gemm_skinny_kernel<__half>);
-  int resident = 0;
-  if (int rc = blocks_per_sm(kern, kThreads, smem, &resident)) return rc;
-  if (resident < 1) return NPB_ERR_TOO_LARGE;
   CUtensorMap map_w, map_x;
   const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (int rc = make_tensor_map_2d(&map_w, type, 2, w, N, K, BN, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  if (int rc = make_tensor_map_2d(&map_x, type, 2, x, M, K, p.rows, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tensor_map_2d(&map_x, type, 2, x, M, K, p.rows / cg, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)row_tiles);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = 1024 + kHead + ring;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = p.split;
+  attr.val.clusterDim.x = p.split * cg;
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (bf16) NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_skinny_kernel<__nv_bfloat16>, map_w, map_x, p));
-  else NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_skinny_kernel<__half>, map_w, map_x, p));
-  NPB_LAUNCH_CHECK();
-  return NPB_OK;
+  if (bf16)
+    return pair ? launch_skinny<__nv_bfloat16, true>(cfg, map_w, map_x, p)
+                : launch_skinny<__nv_bfloat16, false>(cfg, map_w, map_x, p);
+  return pair ? launch_skinny<__half, true>(cfg, map_w, map_x, p) : launch_skinny<__half, false>(cfg, map_w, map_x, p);
 }
 
 // Reads and clears the give-up record (npb_gemm_device_status collects it).
