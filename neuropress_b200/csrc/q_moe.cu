@@ -6,10 +6,9 @@
 //   y_t     = T( sum_{e in S_t} D_e h_te )                         kernel 2: routing, down, sum
 //   W[n, k] = (q[n, k] - z) * s  in fp32, z and s per group of k (z = 8 without a zero point)
 //
-// Each active expert's codes are read once; HBM-bound (0.56 bytes per weight at group 32).  Both kernels
-// route by themselves (a warp per token, every CTA alike: a microsecond, no hand-over between kernels),
-// and the second is launched with programmatic serialisation, so it routes and fetches its first
-// weights under the end of the first.
+// Each active expert's codes are read once; HBM-bound (0.56 bytes per weight at group 32).  Every CTA of the first
+// kernel routes by itself (a warp per token); the second reads the outcome with h.  It is launched with
+// programmatic serialisation, so its CTAs are set up when the first kernel ends.
 //
 // Product: mma.sync.m16n8k16 in fp16 with the weights as the A operand (16 rows) built in registers.  A code
 // q becomes 1024 + q or, four bits higher in the mantissa, 1024 + 16 q with one bit operation per two
@@ -58,6 +57,8 @@ constexpr int kMaxTopK = 16;
 constexpr int kMaxUnits = kMaxTokens * kMaxTopK;
 constexpr int kMaxWidth = 16384;  // of H and I: two tokens of H in shared memory next to the rings
 
+struct Units;
+
 struct MoeWeight {
   const uint8_t* codes;
   const __half* scale;
@@ -74,6 +75,7 @@ struct MoeParams {
   int T, E, H, I, top_k, renormalize;
   MoeWeight gate, up, down;
   uint8_t* h;      // [pair of tokens of a unit][I / 32] records
+  Units* units;
   void* y;
   uint64_t wait_ns;
 };
@@ -82,14 +84,20 @@ struct MoeParams {
 constexpr int kRecord = 160;
 
 // ---- routing ---------------------------------------------------------------------------------
+// The work lists: a unit is up to NT tokens of one expert.
+struct Units {
+  int n;
+  int unused[3];
+  uint32_t mask[kMaxUnits];      // the unit's tokens
+  uint16_t expert[kMaxUnits];
+  uint16_t slot[kMaxUnits];      // row of h of its first pair
+};
+
 struct Routing {
   uint32_t mask[kMaxExperts];            // tokens of each expert
   float weight[kMaxTokens][kMaxTopK];
   uint16_t id[kMaxTokens][kMaxTopK];     // 0xffff: none
-  uint16_t unit_expert[kMaxUnits];
-  uint32_t unit_mask[kMaxUnits];         // its tokens
-  uint16_t unit_slot[kMaxUnits];         // row of h of its first pair
-  int n_units;
+  Units units;
 };
 
 __device__ __forceinline__ float load_logit(const MoeParams& p, int64_t i) {
@@ -123,7 +131,7 @@ __device__ void choose(const MoeParams& p, Routing& r) {
     all = warp_sum(all);
     // a row with NaN or +inf has NaN weights (all is NaN); a row of -inf alone is routed nowhere
     const bool nowhere = m == -INFINITY && !__any_sync(0xffffffffu, nan);
-    float chosen = 0.f;
+    uint32_t mine = 0, mine_e = 0;  // lane j: the j-th largest
     for (int j = 0; j < p.top_k; ++j) {
       uint32_t best = 0;
       int at = 0;
@@ -135,19 +143,19 @@ __device__ void choose(const MoeParams& p, Routing& r) {
 #pragma unroll
       for (int i = 0; i < PER_LANE; ++i)
         if (i * 32 + lane == (int)e) key[i] = 0;
-      const float l = key_value(top);
-      const float w = expf(l - m);
-      chosen += w;
-      if (lane == 0) {
-        const bool none = nowhere || (l == -INFINITY && all == all);  // probability 0: not read
-        r.id[t][j] = none ? 0xffffu : (uint16_t)e;
-        r.weight[t][j] = w;
-        if (!none) atomicOr(&r.mask[e], 1u << t);
+      if (lane == j) {
+        mine = top;
+        mine_e = e;
       }
     }
-    __syncwarp();
-    const float norm = p.renormalize ? (all != all ? all : chosen) : all;
-    for (int j = lane; j < p.top_k; j += 32) r.weight[t][j] /= norm;
+    const float l = key_value(mine), w = lane < p.top_k ? expf(l - m) : 0.f;
+    const float norm = p.renormalize ? (all != all ? all : warp_sum(w)) : all;
+    if (lane < p.top_k) {
+      const bool none = nowhere || (l == -INFINITY && all == all);  // probability 0: not read
+      r.id[t][lane] = none ? 0xffffu : (uint16_t)mine_e;
+      r.weight[t][lane] = w / norm;
+      if (!none) atomicOr(&r.mask[mine_e], 1u << t);
+    }
   }
 }
 
@@ -178,15 +186,15 @@ __device__ void route(const MoeParams& p, Routing& r) {
         const int at = units + iu - u + i;
         uint32_t rest = m;
         for (int j = 0; j < NT && rest; ++j) rest &= rest - 1;
-        r.unit_expert[at] = (uint16_t)e;
-        r.unit_mask[at] = m & ~rest;
-        r.unit_slot[at] = (uint16_t)(slots + in - pairs + i * (NT / 2));
+        r.units.expert[at] = (uint16_t)e;
+        r.units.mask[at] = m & ~rest;
+        r.units.slot[at] = (uint16_t)(slots + in - pairs + i * (NT / 2));
         m = rest;
       }
       units += __shfl_sync(0xffffffffu, iu, 31);
       slots += __shfl_sync(0xffffffffu, in, 31);
     }
-    if (lane == 0) r.n_units = units;
+    if (lane == 0) r.units.n = units;
   }
   __syncthreads();
 }
@@ -508,8 +516,16 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   }
   route<NT>(p, r);
 
+  if (blockIdx.x == 0) {  // for kernel 2
+    if (tid == 0) p.units->n = r.units.n;
+    for (int i = tid; i < r.units.n; i += kUpThreads) {
+      p.units->mask[i] = r.units.mask[i];
+      p.units->expert[i] = r.units.expert[i];
+      p.units->slot[i] = r.units.slot[i];
+    }
+  }
   const int tiles = p.I / kUpRows;
-  const int64_t items = (int64_t)tiles * r.n_units;
+  const int64_t items = (int64_t)tiles * r.units.n;
   const int first = (int)(items * blockIdx.x / gridDim.x), last = (int)(items * (blockIdx.x + 1) / gridDim.x);
   const int mt = warp & 1, ks = warp >> 1;
   const int s_first = n_steps * ks / kUpSlices, s_last = n_steps * (ks + 1) / kUpSlices;
@@ -528,7 +544,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   auto f_start = [&] {
     if (f_item < last) {
       const int u = f_item / tiles;
-      f_row = r.unit_expert[u] * p.I + (f_item - u * tiles) * kUpRows + mt * 16;
+      f_row = r.units.expert[u] * p.I + (f_item - u * tiles) * kUpRows + mt * 16;
     }
   };
   f_start();
@@ -564,49 +580,59 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   bool ok = true;
   for (int item = first; item < last; ++item) {
     const int u = item / tiles, i0 = (item - u * tiles) * kUpRows;
-    const int e = r.unit_expert[u];
+    const int e = r.units.expert[u];
     if (u != unit) {
       if (tid < NT) x_top[tid] = 0;
       __syncthreads();  // everybody is through with the unit before
       unit = u;
-      const uint32_t mask = r.unit_mask[u];
+      const uint32_t mask = r.units.mask[u];
       n = __popc(mask);
-      // the unit's tokens, a thread takes eight elements (columns of an mma past the last token hold what was there:
-      // nothing reads their sums): the largest magnitude, then the stored values
-#pragma unroll 1
-      for (int pass = 0; pass < 2; ++pass) {
+      // the unit's tokens, eight elements of each to a thread (columns of an mma past the last token hold what was
+      // there: nothing reads their sums): the largest magnitude of each, then the stored values.  Rows of up to 4096
+      // stay in registers between the two.
+      uint4 raw[NT] = {};
+      auto load = [&](int j) {
         uint32_t m = mask;
+#pragma unroll
+        for (int i = 0; i < NT; ++i, m &= m - 1) {
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (i < n && j < n_blk * 4)
+            raw[i] = __ldg(reinterpret_cast<const uint4*>(p.x) + (int64_t)(__ffs(m) - 1) * (n_blk * 4) + j);
+        }
+      };
+      const bool bf16 = p.dtype == NPB_BF16, held = blocks * 4 <= kUpThreads;
+      float top[NT] = {};
 #pragma unroll 1
-        for (int i = 0; i < n; ++i, m &= m - 1) {
-          const uint4* src = reinterpret_cast<const uint4*>(p.x) + (int64_t)(__ffs(m) - 1) * (n_blk * 4);
-          float f = 1.f;
-          if (pass) {
-            f = power_below(__uint_as_float(x_top[i]));
-            if (tid == 0) x_f[i] = f;
-          }
-          float top = 0.f;
-          for (int j0 = 0; j0 < blocks * 4; j0 += kUpThreads) {  // whole warps
-            const int j = j0 + tid;
-            uint4 raw = make_uint4(0, 0, 0, 0);
-            if (j < n_blk * 4) raw = __ldg(src + j);
-            if (pass == 0) {
-              top = fmaxf(top, p.dtype == NPB_BF16 ? largest<__nv_bfloat16>(raw) : largest<__half>(raw));
-              continue;
-            }
+      for (int j = tid; j < blocks * 4; j += kUpThreads) {
+        load(j);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          top[i] = fmaxf(top[i], bf16 ? largest<__nv_bfloat16>(raw[i]) : largest<__half>(raw[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top[i]));
+        if (lane == 0 && i < n) atomicMax(&x_top[i], bits);
+      }
+      __syncthreads();
+      if (tid < n) x_f[tid] = power_below(__uint_as_float(x_top[tid]));
+#pragma unroll 1
+      for (int j0 = 0; j0 < blocks * 4; j0 += kUpThreads) {  // whole warps
+        const int j = j0 + tid;
+        if (!held) load(j);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (i < n) {
+            const float by = 1.f / power_below(__uint_as_float(x_top[i]));
             uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
             float* to_m = reinterpret_cast<float*>(dyn + at.m) + (i / 2 * (blocks + 1) + (j >> 2)) * 4 + (i & 1);
             float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + (i / 2 * blocks + (j >> 2)) * 2 + (i & 1) : nullptr;
             const bool write = j < blocks * 4;
-            if (p.dtype == NPB_BF16) store_operand<__nv_bfloat16>(raw, 1.f / f, to, to_m, to_s2, write, ASYM);
-            else store_operand<__half>(raw, 1.f / f, to, to_m, to_s2, write, ASYM);
+            if (bf16) store_operand<__nv_bfloat16>(raw[i], by, to, to_m, to_s2, write, ASYM);
+            else store_operand<__half>(raw[i], by, to, to_m, to_s2, write, ASYM);
           }
-          if (pass == 0) {
-            const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-            if (lane == 0) atomicMax(&x_top[i], bits);
-          }
-        }
-        __syncthreads();
       }
+      __syncthreads();
     }
     float acc[2][4] = {};
     int w_s = 0, w_next = s_first;
@@ -651,7 +677,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
       }
       gate *= x_f[warp];
       up *= x_f[warp];
-      uint32_t m = r.unit_mask[u];
+      uint32_t m = r.units.mask[u];
       for (int i = 0; i < warp; ++i) m &= m - 1;
       const int token = __ffs(m) - 1;
       float weight = 0.f;
@@ -665,7 +691,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
       const bool is_odd = lane & 1;  // pair (lane & 3) of its word
       const __half v = __float2half_rn(h * ((is_odd ? 0.0625f : 1.f) / f));
       const float even = warp_sum(is_odd ? 0.f : __half2float(v)), odd = warp_sum(is_odd ? __half2float(v) : 0.f);
-      uint8_t* rec = p.h + ((int64_t)(r.unit_slot[u] + warp / 2) * (p.I / 32) + i0 / 32) * kRecord;
+      uint8_t* rec = p.h + ((int64_t)(r.units.slot[u] + warp / 2) * (p.I / 32) + i0 / 32) * kRecord;
       reinterpret_cast<__half*>(rec)[(warp & 1) * 32 + (lane & 24) + (lane & 3) * 2 + ((lane >> 2) & 1)] = v;
       if (lane == 0) {
         float* to = reinterpret_cast<float*>(rec + 128) + (warp & 1);
@@ -716,7 +742,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
   using Rg = Ring<G, kDownTiles, ASYM, MODE>;
   extern __shared__ uint8_t dyn_raw[];
   uint8_t* dyn = dyn_raw + ((1024u - (sm100::smem_u32(dyn_raw) & 1023u)) & 1023u);
-  __shared__ Routing r;
+  __shared__ Units u;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -742,10 +768,17 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     for (int i = 0; i < stages; ++i) sm100::mbar_init(&bars[i], 1);
     sm100::fence_barrier_init();
   }
-  route<NT>(p, r);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // kernel 1's lists and h are written
+  const int n_units = __ldcg(&p.units->n);
+  for (int i = tid; i < n_units; i += kDownThreads) {
+    u.mask[i] = __ldcg(&p.units->mask[i]);
+    u.expert[i] = __ldcg(&p.units->expert[i]);
+    u.slot[i] = __ldcg(&p.units->slot[i]);
+  }
+  __syncthreads();
 
   // (unit, step) pairs in a row, an equal share of consecutive ones per warp of the cluster
-  const int64_t total = (int64_t)r.n_units * n_steps;
+  const int64_t total = (int64_t)n_units * n_steps;
   const int share = rank * kDownWarps + warp, shares = kDownSplit * kDownWarps;
   const int first = (int)(total * share / shares), last = (int)(total * (share + 1) / shares);
   const int lane_blk = t / (4 / G);
@@ -761,7 +794,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
   // a run of windows is what the warp does of one unit
   int f_at = first, f_u = first_u, f_s = first_s, f_stage = 0, f_window = 0, f_next = first_s;
   auto fetch_weights = [&] {
-    const int row0 = r.unit_expert[f_u] * p.H + j0;
+    const int row0 = u.expert[f_u] * p.H + j0;
     if (lane == 0) {
       sm100::mbar_arrive_expect_tx(&bars[f_stage], Rg::kCodes);
       sm100::tma_load_2d(dyn + code_ring + f_stage * Rg::kCodes, &map, &bars[f_stage], f_s * 64, row0);
@@ -782,8 +815,8 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     part_src[i] = pair * n_blk * kRecord + (c - pair * 4 * kPieces) * 16;
   }
   auto fetch_records = [&] {  // blocks 4 f_s .. + 4 of the unit's tokens; zeros past n_blk
-    const uint8_t* rec = p.h + ((int64_t)r.unit_slot[f_u] * n_blk + f_s * 4) * kRecord;
-    const int pieces = (__popc(r.unit_mask[f_u]) + 1) / 2 * 4 * kPieces;
+    const uint8_t* rec = p.h + ((int64_t)u.slot[f_u] * n_blk + f_s * 4) * kRecord;
+    const int pieces = (__popc(u.mask[f_u]) + 1) / 2 * 4 * kPieces;
     const uint32_t to = base + rest_ring + f_stage * at.stage + Rg::kWindow + lane * 16;
     const int whole = (n_blk - f_s * 4) * kPieces;  // pieces of a pair that exist
 #pragma unroll
@@ -808,7 +841,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
   float acc[kDownTiles][4] = {};
   int unit = -1;
   auto flush = [&] {
-    uint32_t m = unit >= 0 ? r.unit_mask[unit] : 0u;
+    uint32_t m = unit >= 0 ? u.mask[unit] : 0u;
     for (int i = 0; i < 2 * t; ++i) m &= m - 1;  // of this lane's two tokens
     const int token[2] = {__ffs(m) - 1, __ffs(m & (m - 1)) - 1};
 #pragma unroll
@@ -825,56 +858,44 @@ moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, cons
     __syncwarp();
   };
 
-  // the first weights are under way before kernel 1 ends; h exists only after it
-  for (int i = 0; i < stages; ++i) {
-    if (f_at < last) fetch_weights();
-    advance();
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  f_at = first;
-  f_u = first_u;
-  f_s = first_s;
-  f_stage = 0;
-  for (int i = 0; i < stages; ++i) {
-    if (f_at < last) fetch_records();
-    advance();
-  }
   int c_u = first_u, c_s = first_s, stage = 0, window = -1, w_s = 0, w_next = first_s;
   uint32_t parity = 0;
   bool ok = true;
-  for (int q = first; q < last; ++q) {
-    if (c_u != unit) {
-      flush();
-      unit = c_u;
+  for (int q = first - stages; q < last; ++q) {
+    if (q >= first) {
+      if (c_u != unit) {
+        flush();
+        unit = c_u;
+      }
+      ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
+      cp_async_wait(stages - 1);
+      __syncwarp();
+      if (c_s == w_next) {
+        if (++window == stages) window = 0;
+        w_s = c_s;
+        w_next = Rg::next_window(p.down, c_s);
+      }
+      const int index = Rg::index_of(p.down, c_s, w_s, g, n_group);
+      const uint8_t* side = sides + stage * at.stage;
+      add_step<G, kDownTiles, ASYM, MODE, true, kRecord, kRecord, kRecord>(acc, dyn + code_ring + stage * Rg::kCodes,
+                                                                  dyn + rest_ring + window * at.stage, index, operand + stage * operand_stage,
+                                                                  Sides{side, side + 16, side + 24}, g, t, c_s, n_blk,
+                                                                  p.down);
+      __syncwarp();
+      if (++c_s == n_steps) {
+        c_s = w_next = 0;
+        ++c_u;
+      }
+      if (++stage == stages) {
+        stage = 0;
+        parity ^= 1;
+      }
     }
-    ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
-    cp_async_wait(stages - 1);
-    __syncwarp();
-    if (c_s == w_next) {
-      if (++window == stages) window = 0;
-      w_s = c_s;
-      w_next = Rg::next_window(p.down, c_s);
-    }
-    const int index = Rg::index_of(p.down, c_s, w_s, g, n_group);
-    const uint8_t* side = sides + stage * at.stage;
-    add_step<G, kDownTiles, ASYM, MODE, true, kRecord, kRecord, kRecord>(acc, dyn + code_ring + stage * Rg::kCodes,
-                                                                dyn + rest_ring + window * at.stage, index, operand + stage * operand_stage,
-                                                                Sides{side, side + 16, side + 24}, g, t, c_s, n_blk,
-                                                                p.down);
-    __syncwarp();
     if (f_at < last) {
       fetch_weights();
       fetch_records();
     }
     advance();
-    if (++c_s == n_steps) {
-      c_s = w_next = 0;
-      ++c_u;
-    }
-    if (++stage == stages) {
-      stage = 0;
-      parity ^= 1;
-    }
   }
   flush();
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -924,10 +945,10 @@ int make_code_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int64_t 
 
 // Ring stages that fit next to the rest (2..4; 0: not even two do).
 template <typename Bytes>
-int pick_stages(Bytes bytes, int ctas_per_sm) {
+int pick_stages(Bytes bytes, int static_bytes, int ctas_per_sm) {
   const int cap = ctas_per_sm == 1 ? max_dynamic_smem() : (max_dynamic_smem() - 1024) / ctas_per_sm - 1024;
   int stages = kMaxStages;
-  while (stages >= 2 && bytes(stages) + (int)sizeof(Routing) + 256 > cap) --stages;
+  while (stages >= 2 && bytes(stages) + static_bytes > cap) --stages;
   return stages >= 2 ? stages : 0;
 }
 
@@ -938,7 +959,7 @@ int up_bytes(const MoeParams& p, int g, int stages) {
                   window_bytes(32, p.gate.zp != nullptr, mode_of(p.gate, p.H / 32)), stages).bytes;
 }
 int up_stages(const MoeParams& p, int g) {
-  return pick_stages([&](int n) { return up_bytes(p, g, n); }, 1);
+  return pick_stages([&](int n) { return up_bytes(p, g, n); }, (int)sizeof(Routing) + 256, 1);
 }
 int down_bytes(const MoeParams& p, int g, int stages) {
   return DownLayout(p.T, 8 / g, kDownRows * 64,
@@ -946,8 +967,8 @@ int down_bytes(const MoeParams& p, int g, int stages) {
 }
 int down_stages(const MoeParams& p, int g) {
   auto bytes = [&](int n) { return down_bytes(p, g, n); };
-  const int two = g == 1 ? 0 : pick_stages(bytes, 2);  // two CTAs on an SM where they fit
-  return two ? two : pick_stages(bytes, 1);
+  const int two = g == 1 ? 0 : pick_stages(bytes, (int)sizeof(Units) + 256, 2);  // two CTAs on an SM where they fit
+  return two ? two : pick_stages(bytes, (int)sizeof(Units) + 256, 1);
 }
 
 template <int G, bool ASYM, int MODE>
@@ -1052,7 +1073,7 @@ int q_moe_device_status(int* host_out) {
 
 int64_t q_moe_workspace_bytes(int64_t T, int top_k, int64_t I) {
   if (T < 0 || top_k <= 0 || I <= 0 || T > kMaxTokens || top_k > kMaxTopK || I % 32 != 0) return 0;
-  return T * top_k * (I / 32) * kRecord;  // a pair of tokens of an expert is at least one of the T * top_k
+  return (int64_t)sizeof(Units) + T * top_k * (I / 32) * kRecord;  // a pair of tokens of an expert is at least one of the T * top_k
 }
 
 int q_moe(const void* x, int dtype, const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t H, int64_t I,
@@ -1082,7 +1103,8 @@ int q_moe(const void* x, int dtype, const void* logits, int logits_dtype, int64_
   p.T = (int)T; p.E = (int)E; p.H = (int)H; p.I = (int)I;
   p.top_k = top_k;
   p.renormalize = renormalize != 0;
-  p.h = static_cast<uint8_t*>(workspace);
+  p.units = static_cast<Units*>(workspace);
+  p.h = static_cast<uint8_t*>(workspace) + sizeof(Units);
   p.y = y;
   p.wait_ns = wait_limit_ns();
   return launch_tokens(p, st);
