@@ -252,9 +252,9 @@ def require_cuda(name: str, *tensors: torch.Tensor | None) -> None:
         if not t.is_contiguous():
             raise RuntimeError(f"{name}: all tensors must be contiguous.")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{name}: tensors are on different devices ({dev} vs {t.device}).")
+            dev = t.get_device()
+        elif t.get_device() != dev:
+            raise RuntimeError(f"{name}: tensors are on different devices (cuda:{dev} vs {t.device}).")
 
 
 def vq_struct(
@@ -307,13 +307,8 @@ def q_struct(codes: torch.Tensor, scale: torch.Tensor, zero_point: torch.Tensor 
         raise RuntimeError("codes must be uint8.")
     if scale.dtype != torch.float16 or (zero_point is not None and zero_point.dtype != torch.float16):
         raise RuntimeError("scale / zero_point must be float16.")
-    s = QWeightStruct()
-    s.codes = codes.data_ptr()
-    s.scale = scale.data_ptr()
-    s.zero_point = _ptr(zero_point)
-    s.nbits = int(nbits)
-    s.group_size = int(group_size)
-    return s
+    return QWeightStruct(codes.data_ptr(), scale.data_ptr(), None if zero_point is None else zero_point.data_ptr(),
+                         int(nbits), int(group_size))
 
 
 def gemm_device_status() -> int:

@@ -9,13 +9,17 @@
 // HBM once.  All sums are fp32; l - m is formed before the multiplication by log2(e), so rows with a
 // large common offset lose nothing.  Bound by HBM for many rows, by latency for a few.
 //
-// The n largest without a second pass: the n-th largest of the 256 THREAD maxima is a lower bound of
-// the n-th largest element, and only a handful of elements reach it.  The about n threads whose
-// maximum reaches the bound are re-read (L2), their elements at or above it go to a shared-memory
-// list, and an element's rank in the answer is the number of larger (value, index) keys in the list --
-// no order of arrival enters the result.  Rows where that list overflows (masked or constant rows: the
-// bound ties with most of the row) find the exact n-th value by bisection over the ordered bits of the
-// values and take the ties in index order.
+// The n largest without a second pass: if every full warp's q-th largest THREAD maximum is at least b, with q = n /
+// warps rounded up, n elements are at least b, and only a few dozen elements are.  The threads whose maximum
+// reaches the least of those q-th largest are re-read (L2), their elements at or above it go to a shared-memory
+// list, and an element's rank in the answer is the number of larger (value, index) keys in the list -- no order of
+// arrival enters the result.  Rows where that list overflows (masked or constant rows: the bound ties with most of
+// the row) find the exact n-th value by bisection over the ordered bits of the values and take the ties in index
+// order.  The CTAs of a cluster meet with sorted lists, where a rank is a binary search in each.
+//
+// Per element of a 16-bit row: one unpacking, half an instruction each for the maximum (on packed pairs), l - m, its
+// scaling, and the two sums (packed fp32), one ex2.  The exponentials alone would take 0.7 of the time that HBM
+// needs for them.
 #include "common.cuh"
 #include "order_key.cuh"
 #include "tcgen05.cuh"
@@ -76,13 +80,61 @@ __device__ __forceinline__ typename Tile<T>::Vec load_vec(const T* p) {
   return *reinterpret_cast<const typename Tile<T>::Vec*>(&r);
 }
 
-// Adds N elements to a part.  The product e * d is 0 * -inf = NaN for a masked (-inf) element; such a
-// tile (u is NaN, s is not) is summed again with d clamped, so that the others pay nothing.
-template <int N>
-__device__ __forceinline__ void add_elements(Part& p, const float (&f)[N]) {
-  float tm = f[0];
+// Two floats in a register pair, for the packed fp32 instructions.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack(const F2& x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 add2(const F2& a, const F2& b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(const F2& a, const F2& b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(const F2& a, const F2& b, const F2& c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Element pairs of a vector as floats, and the largest element (NaN only if every element is).
+template <typename T>
+__device__ __forceinline__ F2 pair_of(const typename Tile<T>::Vec& q, int i) {
+  return pack(to_f32(q.e[2 * i]), to_f32(q.e[2 * i + 1]));
+}
+__device__ __forceinline__ float largest(const Tile<float>::Vec& q) {
+  return fmaxf(fmaxf(q.e[0], q.e[1]), fmaxf(q.e[2], q.e[3]));
+}
+__device__ __forceinline__ float largest(const Tile<__half>::Vec& q) {
+  const __half2* h = reinterpret_cast<const __half2*>(q.e);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float largest(const Tile<__nv_bfloat16>::Vec& q) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(q.e);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+// Adds N vectors to a part.  The product e * d is 0 * -inf = NaN for a masked (-inf) element; such a tile (u is NaN,
+// s is not) is summed again with d clamped, so that the others pay nothing.
+template <typename T, int N>
+__device__ __forceinline__ void add_vectors(Part& p, const typename Tile<T>::Vec (&q)[N]) {
+  constexpr int PAIRS = Tile<T>::EPV / 2;
+  float tm = largest(q[0]);
 #pragma unroll
-  for (int i = 1; i < N; ++i) tm = fmaxf(tm, f[i]);
+  for (int i = 1; i < N; ++i) tm = fmaxf(tm, largest(q[i]));
   if (tm > p.m) {
     const float d = fmaxf(p.m - tm, -1e20f), c = ex2(d * kLog2e);
     p.u = c * (p.u + d * p.s);
@@ -90,30 +142,47 @@ __device__ __forceinline__ void add_elements(Part& p, const float (&f)[N]) {
     p.m = tm;
   }
   const float ref = p.m == -INFINITY ? 0.f : p.m;
-  float s = 0.f, u = 0.f;
+  const F2 less = pack(-ref, -ref), scale = pack(kLog2e, kLog2e);
+  F2 s2 = pack(0.f, 0.f), u2 = s2;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = f[i] - ref;
-    const float e = ex2(d * kLog2e);
-    s += e;
-    u = fmaf(e, d, u);
-  }
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int k = 0; k < PAIRS; ++k) {
+      const F2 d = add2(pair_of<T>(q[i], k), less);
+      float a, b;
+      unpack(mul2(d, scale), a, b);
+      const F2 e = pack(ex2(a), ex2(b));
+      s2 = add2(s2, e);
+      u2 = fma2(e, d, u2);
+    }
+  float s, s_hi, u, u_hi;
+  unpack(s2, s, s_hi);
+  unpack(u2, u, u_hi);
+  s += s_hi;
+  u += u_hi;
   if (u != u) {
     u = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = f[i] - ref;
-      u = fmaf(ex2(d * kLog2e), fmaxf(d, -1e20f), u);
-    }
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < 2 * PAIRS; ++k) {
+        const float d = to_f32(q[i].e[k]) - ref;
+        u = fmaf(ex2(d * kLog2e), fmaxf(d, -1e20f), u);
+      }
   }
   p.s += s;
   p.u += u;
 }
 
+// A part of one element.
+__device__ __forceinline__ Part part_of(float f) {
+  const float d = f - (f == -INFINITY ? 0.f : f);  // 0, or NaN for NaN and +inf
+  return {f == f ? f : -INFINITY, f == -INFINITY ? 0.f : ex2(d), f == -INFINITY ? 0.f : d};
+}
+
 struct Shared {
   Part warp_part[kWarps];
   Part parts[kMaxSplit];             // rank 0: one per CTA of the cluster
-  uint32_t thread_max[kThreads];
   uint32_t bound;                    // key the n-th largest element is known to reach
   int n_hot, n_list;
   int hot[kThreads];                 // threads whose maximum reaches the bound
@@ -218,29 +287,19 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
   }
 
   Part p{-INFINITY, 0.f, 0.f};
+  const T* vectors = row + head;
   int v = v0 + tid;
   for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
     typename Tile<T>::Vec q[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) q[i] = load_vec(row + head + (int64_t)(v + i * kThreads) * EPV);
-    float f[kUnroll * EPV];
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) f[i * EPV + e] = to_f32(q[i].e[e]);
-    add_elements(p, f);
+    for (int i = 0; i < kUnroll; ++i) q[i] = load_vec(vectors + (int64_t)(v + i * kThreads) * EPV);
+    add_vectors<T>(p, q);
   }
   for (; v < v1; v += kThreads) {
-    const typename Tile<T>::Vec q = load_vec(row + head + (int64_t)v * EPV);
-    float f[EPV];
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) f[e] = to_f32(q.e[e]);
-    add_elements(p, f);
+    const typename Tile<T>::Vec q[1] = {load_vec(vectors + (int64_t)v * EPV)};
+    add_vectors<T>(p, q);
   }
-  if (odd >= 0) {
-    const float f[1] = {to_f32(row[odd])};
-    add_elements(p, f);
-  }
+  if (odd >= 0) p = merge(p, part_of(to_f32(row[odd])));
 
   const bool mine = v0 + tid < v1 || odd >= 0;
   if (top_n > 0) {
@@ -249,20 +308,24 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
     const int count = (v1 - v0) * EPV + (rank == 0 ? head + (V - tail) : 0);
     const int need = min(top_n, count);
     const uint32_t my_max = mine ? order_key(p.m) : 0u;
-    sh.thread_max[tid] = my_max;
-    if (tid == 0) { sh.bound = 0; sh.n_hot = 0; sh.n_list = 0; }
-    __syncthreads();
-    int larger = 0, equal_before = 0;
-    for (int i = 0; i < kThreads; i += 4) {
-      const uint4 o = *reinterpret_cast<const uint4*>(&sh.thread_max[i]);
-      larger += (o.x > my_max) + (o.y > my_max) + (o.z > my_max) + (o.w > my_max);
-      equal_before += (o.x == my_max && i < tid) + (o.y == my_max && i + 1 < tid) + (o.z == my_max && i + 2 < tid) +
-                      (o.w == my_max && i + 3 < tid);
+    const int full = min(v1 - v0, kThreads) / 32;  // warps of which every thread has elements
+    if (tid == 0) {
+      sh.bound = full ? 0xffffffffu : 0u;          // none: everything is a candidate
+      sh.n_hot = 0;
+      sh.n_list = 0;
     }
-    if (larger + equal_before == need - 1) sh.bound = my_max;  // the need-th largest thread maximum
+    __syncthreads();
+    if (warp < full) {
+      uint32_t left = my_max, nth = 0;
+      for (int q = (need + full - 1) / full; q > 0; --q) {
+        nth = __reduce_max_sync(0xffffffffu, left);
+        const uint32_t who = __ballot_sync(0xffffffffu, left == nth);
+        if (lane == __ffs(who) - 1) left = 0;
+      }
+      if (lane == 0) atomicMin(&sh.bound, nth);
+    }
     __syncthreads();
     const uint32_t bound = sh.bound;
-    // bound 0: fewer threads than `need` hold an element; everything is a candidate
     if (my_max != 0 && my_max >= bound) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
     __syncthreads();
     const int n_hot = sh.n_hot, per = (v1 - v0 + kThreads - 1) / kThreads + 1;  // + the odd element
@@ -373,8 +436,15 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
       const unsigned long long key = sh.best[(i / top_n) * kMaxTop + i % top_n];
       if (key == 0) continue;
       int pos = 0;
-      for (int c = 0; c < split; ++c)
-        for (int j = 0; j < top_n; ++j) pos += sh.best[c * kMaxTop + j] > key;
+#pragma unroll
+      for (int c = 0; c < kMaxSplit; ++c)
+        if (c < split) {  // keys of a CTA that are larger: its list is in descending order
+          int n = 0;
+#pragma unroll
+          for (int step = kMaxTop; step > 0; step >>= 1)
+            if (n + step <= top_n && sh.best[c * kMaxTop + n + step - 1] > key) n += step;
+          pos += n;
+        }
       if (pos < top_n) {
         top_ids[r * top_n + pos] = (int64_t)(uint32_t)~(uint32_t)key;
         top_logprobs[r * top_n + pos] = log_p(key_value((uint32_t)(key >> 32)));
@@ -386,7 +456,7 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
 // CTAs per row: as many as keep the GPU busy with few rows, each with a slice worth its start.
 int pick_split(int64_t R, int64_t V) {
   int split = 1;
-  while (split < kMaxSplit && R * split * 2 <= (int64_t)sm_count() * 4 && V / (split * 2) >= 2048) split *= 2;
+  while (split < kMaxSplit && R * split * 2 <= (int64_t)sm_count() * 6 && V / (split * 2) >= 2048) split *= 2;
   return split;
 }
 

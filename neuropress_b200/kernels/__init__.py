@@ -593,11 +593,11 @@ def q_linear(x: torch.Tensor, w_pack: torch.Tensor, scale: torch.Tensor, nbits: 
 # ---------------------------------------------------------------------------
 
 
-def _moe_weight(name: str, weight: tuple, e: int, rows: int, k: int, group_size: int):
+def _moe_weight(name: str, weight: tuple, shape: tuple, group_size: int):
     codes, scale, zero_point = weight
-    if tuple(codes.shape) != (e, rows, k // 2):
-        raise RuntimeError(f"q_moe: the codes of {name} must be [{e}, {rows}, {k // 2}], got {list(codes.shape)}.")
-    n_groups = e * rows * (k // group_size)
+    if codes.shape != shape:
+        raise RuntimeError(f"q_moe: the codes of {name} must be {list(shape)}, got {list(codes.shape)}.")
+    n_groups = shape[0] * shape[1] * (shape[2] * 2 // group_size)
     if scale.numel() != n_groups or (zero_point is not None and zero_point.numel() != n_groups):
         raise RuntimeError(f"q_moe: scale / zero_point of {name} must have {n_groups} elements.")
     return _cabi.q_struct(codes, scale, zero_point, 4, group_size)
@@ -631,8 +631,9 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
                            f"{_cabi.MOE_MAX_EXPERTS}].")
     if (gate[2] is None) != (up[2] is None):
         raise RuntimeError("q_moe: gate and up must both have zero points or both have none.")
-    structs = (_moe_weight("gate", gate, e, i, h, group_size), _moe_weight("up", up, e, i, h, group_size),
-               _moe_weight("down", down, e, h, i, group_size))
+    into = (e, i, h // 2)
+    structs = (_moe_weight("gate", gate, into, group_size), _moe_weight("up", up, into, group_size),
+               _moe_weight("down", down, (e, h, i // 2), group_size))
     _cabi.require_cuda("q_moe", x, router_logits, *gate, *up, *down)
     lib = _cabi.load_library()
     code, logit_code = _cabi.dtype_code(x.dtype), _cabi.dtype_code(router_logits.dtype)
@@ -641,13 +642,14 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
         return y
     n = min(t, _cabi.MOE_MAX_TOKENS)
     size = lib.npb_q_moe_workspace_bytes(n, top_k, i)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    workspace = x.new_empty((size,), dtype=torch.uint8)
     x_step, l_step = h * x.element_size(), e * router_logits.element_size()
+    x_at, l_at, y_at, renorm = x.data_ptr(), router_logits.data_ptr(), y.data_ptr(), int(renormalize)
     with _cabi.on_device(x.device):
+        stream, scratch = _cabi.stream_ptr(), workspace.data_ptr()
         for t0 in range(0, t, n):
-            rc = _launch("npb_q_moe", lib.npb_q_moe, x.data_ptr() + t0 * x_step, code,
-                         router_logits.data_ptr() + t0 * l_step, logit_code, min(n, t - t0), e, h, i, *structs, top_k,
-                         int(renormalize), workspace.data_ptr(), size, y.data_ptr() + t0 * x_step, _cabi.stream_ptr())
+            rc = _launch("npb_q_moe", lib.npb_q_moe, x_at + t0 * x_step, code, l_at + t0 * l_step, logit_code,
+                         min(n, t - t0), e, h, i, *structs, top_k, renorm, scratch, size, y_at + t0 * x_step, stream)
             _cabi.check(rc, "q_moe")
     return y
 
