@@ -15,10 +15,10 @@
 // q becomes 1024 + q or, four bits higher in the mantissa, 1024 + 16 q with one bit operation per two
 // codes; the activations that meet the latter are stored divided by 16.  With x' the stored activations
 //   sum_k (q - z) x = D - 1024 sum_k x' - z sum_k x,   D the mma's sum
-// is applied per 32-wide block, with the weight's scale, in fp32.  Activations are stored as fp16 after division by a power of two, one per token for x and one per
-// 32-block and token for h, so their size does not matter: x loses nothing down to 2^-13 (bf16) or 2^-10
-// (fp16) of the token's largest and at most 2^-21 of the largest below that; h keeps 11 significant bits
-// between the kernels, 1/8 of a bf16 half step.
+// is applied per 32-wide block, with the weight's scale, in fp32.  Activations are stored as fp16 after division by a
+// power of two, one per token for x and one per 32-block and token for h, so their size does not matter: x loses
+// nothing down to 2^-13 (bf16) or 2^-10 (fp16) of the token's largest and at most 2^-21 of the largest below that; h
+// keeps 11 significant bits between the kernels, 1/8 of a bf16 half step.
 //
 // The eight columns of an mma are NT = 8 / G tokens times G neighbouring 32-blocks (G = 4, 2, 1): lane (g, t)
 // of a warp loads G words, the t-th part of G blocks, of rows g and g + 8, so the k slots of an mma hold
@@ -27,15 +27,22 @@
 // sixteen mmas for two 16-row tiles whatever G is (8 cycles of a scheduler's tensor pipe each, measured);
 // G = 4 has the widest loads and the fewest results to scale, G = 1 the most tokens per weight read.
 //
-// Every warp streams its own weights through a ring of steps in shared memory: codes as TMA boxes of 64 bytes x 16
-// rows with the 64-byte swizzle (no bank conflicts when read, no load instructions, nothing in the L1 path),
-// scales and zero points by cp.async as 16- or 32-byte windows that serve several steps.  What is in flight
-// does not depend on registers: register double buffers of the same kernels reached a third of the bandwidth
-// (waiting for one step's loads waits for the next step's too), and cp.async for the codes left the L1 path
-// 72 % busy.  Kernel 1 keeps the tokens of its unit (up to NT tokens of one expert) in shared memory in the
-// order of the mma operands and writes h in that order; kernel 2 brings h along with the weights.  An expert
-// with more tokens than a unit is read again (from L2).  Every sum has a fixed order: results do not depend
-// on scheduling.  Waits on the TMA barriers are bounded like those of the GEMMs.
+// Weights stream through a ring of rounds in shared memory, filled by producer warps: codes as TMA boxes of 64 bytes of
+// k with the 64-byte swizzle (no bank conflicts when read, nothing in the L1 path), scales and zero points as TMA
+// boxes or, where their rows are not aligned, by cp.async.  In a round each of the sixteen consumer warps takes one
+// step of two 16-row tiles.  Kernel 1 keeps the tokens of a unit (up to NT tokens of one expert), or all of them
+// where there are no more than NT, in shared memory in the order of the mma operands and writes h in that order;
+// kernel 2 brings h along with the weights.  An expert with more tokens than a unit is read again (from L2).  Every
+// sum has a fixed order: results do not depend on scheduling.  Waits on the barriers are bounded like those of the
+// GEMMs.
+//
+// What bounds it: the instructions that turn codes into operands.  With the products left out the two kernels move
+// the weights of 4 tokens, 2 of 8 experts, 4096 x 14336 in 82 + 36 us, with the loads left out they compute for
+// 103 + 49 us, together they take 118 + 54 us (floor at the copy bandwidth 83 us); 32 tokens, 8 of 64 experts, 4096 x
+// 1376: 131 + 83 us (floor 92 us); 1 token, 8 of 64, 2048 x 1024: 21 us, of which 9 are launches, routing and fills.
+// Measured and left: register double buffers (a third of the bandwidth: waiting for one step's loads waits for the
+// next step's too); a ring of each warp's own (80-110 more instructions a step: 185 us for the first case, 206 for the
+// second); 32 consumer warps of 64 registers (spills: 242 and 366 us); 16 warps that fetch in turn (190 and 234 us).
 #include <type_traits>
 
 #include "common.cuh"
@@ -66,7 +73,6 @@ struct MoeWeight {
   const __half* zp;  // null: symmetric, z = 8
   int group_shift;   // log2 of the 32-blocks per group, or -1: divide
   int group_blocks;
-  int window;        // steps that a window of groups serves
 };
 
 struct MoeParams {
@@ -75,10 +81,14 @@ struct MoeParams {
   int logits_dtype, dtype;
   int T, E, H, I, top_k, renormalize;
   MoeWeight gate, up, down;
-  uint8_t* h;      // [pair of tokens of a unit][I / 32] records
+  uint8_t* h;      // [pair of tokens of a unit][I / 32, padded to whole steps] records
   Units* units;
   void* y;
   uint64_t wait_ns;
+  int stages;      // of the ring
+  int window;      // bytes of a row's groups in a round
+  int slices;      // kernel 2: of k in a round; 16 / slices warps side by side over the rows
+  int split;       // kernel 2: CTAs of a cluster
 };
 
 // One 32-block of h of two tokens: 32 stored fp16 values of each (64 bytes), then {m0, m1, m0, m1, f0, f1, s2 of both}.
@@ -95,7 +105,6 @@ struct Units {
 };
 
 struct Routing {
-  uint32_t mask[kMaxExperts];            // tokens of each expert
   float weight[kMaxTokens][kMaxTopK];
   uint16_t id[kMaxTokens][kMaxTopK];     // 0xffff: none
   Units units;
@@ -109,7 +118,7 @@ __device__ __forceinline__ float load_logit(const MoeParams& p, int64_t i) {
 
 // The choices of every token, a warp per token; a lane holds experts lane, lane + 32, ...
 template <int PER_LANE>
-__device__ void choose(const MoeParams& p, Routing& r) {
+__device__ void choose(const MoeParams& p, Routing& r, uint32_t* tokens) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   for (int t = warp; t < p.T; t += warps) {
     uint32_t key[PER_LANE];
@@ -155,26 +164,27 @@ __device__ void choose(const MoeParams& p, Routing& r) {
       const bool none = nowhere || (l == -INFINITY && all == all);  // probability 0: not read
       r.id[t][lane] = none ? 0xffffu : (uint16_t)mine_e;
       r.weight[t][lane] = w / norm;
-      if (!none) atomicOr(&r.mask[mine_e], 1u << t);
+      if (!none) atomicOr(&tokens[mine_e], 1u << t);
     }
   }
 }
 
-// All threads of the CTA; ends with a barrier.  A unit is up to NT tokens of one expert.
+// All threads of the CTA; ends with a barrier.  A unit is up to NT tokens of one expert.  `tokens` [kMaxExperts] is
+// scratch that TMA may write afterwards.
 template <int NT>
-__device__ void route(const MoeParams& p, Routing& r) {
+__device__ void route(const MoeParams& p, Routing& r, uint32_t* tokens) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) r.mask[e] = 0;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) tokens[e] = 0;
   __syncthreads();
-  if (p.E <= 64) choose<2>(p, r);
-  else if (p.E <= 128) choose<4>(p, r);
-  else choose<kMaxExperts / 32>(p, r);
+  if (p.E <= 64) choose<2>(p, r, tokens);
+  else if (p.E <= 128) choose<4>(p, r, tokens);
+  else choose<kMaxExperts / 32>(p, r, tokens);
   __syncthreads();
   if (warp == 0) {
     int units = 0, slots = 0;
     for (int base = 0; base < p.E; base += 32) {
       const int e = base + lane;
-      const int n = e < p.E ? __popc(r.mask[e]) : 0;
+      const int n = e < p.E ? __popc(tokens[e]) : 0;
       const int u = (n + NT - 1) / NT, pairs = (n + 1) / 2;
       int iu = u, in = pairs;
 #pragma unroll
@@ -182,7 +192,7 @@ __device__ void route(const MoeParams& p, Routing& r) {
         const int a = __shfl_up_sync(0xffffffffu, iu, o), b = __shfl_up_sync(0xffffffffu, in, o);
         if (lane >= o) { iu += a; in += b; }
       }
-      uint32_t m = n > 0 ? r.mask[e] : 0u;
+      uint32_t m = n > 0 ? tokens[e] : 0u;
       for (int i = 0; i < u; ++i) {
         const int at = units + iu - u + i;
         uint32_t rest = m;
@@ -197,6 +207,7 @@ __device__ void route(const MoeParams& p, Routing& r) {
     }
     if (lane == 0) r.units.n = units;
   }
+  sm100::fence_proxy_async_smem();
   __syncthreads();
 }
 
@@ -209,65 +220,57 @@ __device__ __forceinline__ int group_of(const MoeWeight& w, int blk) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Waits until at most `pending` (1..3) of the committed groups are under way.
-__device__ __forceinline__ void cp_async_wait(int pending) {
-  if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+// The barrier counts one arrival once this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+               : "memory");
 }
 
-// A warp's ring over R 16-row tiles.  A stage holds one step (four 32-blocks of k): per row 64 bytes of codes as TMA's
-// 64-byte swizzle leaves them (16-byte piece c of row r at c ^ (r / 2 mod 4)).  A window holds per row the 16 or 32
-// bytes, from a 16-byte boundary on, with the groups of several steps; there are as many windows as stages: the
-// steps in the ring need no more.  MODE: kOnePerBlock (a group is a block; a step's four values are eight aligned
-// bytes) and kPowerOfTwo (a group is 2^n blocks) take rows of whole 16-byte windows, one for every eight groups;
-// kAny the rest, 32 bytes at a run's first step and every `window`-th after it.
+// How groups come: kOnePerBlock (a group is a block) and kPowerOfTwo (a group is 2^n blocks) have rows of whole 16-byte
+// pieces, which TMA takes; kAny is the rest.
 enum { kAny = 0, kOnePerBlock = 1, kPowerOfTwo = 2 };
 
-template <int G, int R, bool ASYM, int MODE>
-struct Ring {
-  static constexpr int kRows = 16 * R, kWindowRow = MODE == kAny ? 32 : 16;
-  static constexpr int kCodes = kRows * 64;
-  static constexpr int kWindow = kRows * kWindowRow * (ASYM ? 2 : 1);
-  static constexpr int kZeros = kRows * kWindowRow;  // of the zero points in a window
+constexpr int kConsumers = 16;                    // warps
+// Producer warps: one issues TMA, all copy the windows that TMA cannot take (four against one: 111 -> 83 us for 32 tokens
+// of 64 experts 4096 x 1376; without windows to copy the three would only cost, 118 -> 126 us for 4096 -> 14336).
+constexpr int producers(int mode) { return mode == kAny ? 4 : 1; }
+constexpr int threads_of(int mode) { return (kConsumers + producers(mode)) * 32; }
+constexpr int kMaxStages = 4;
 
-  // Tile row of lane group g: G = 2 reads half pieces, which needs every other pair of rows in a phase.
-  __device__ static int row_of(int g) { return G == 2 ? (g & 1) | (g & 2) << 1 | (g & 4) >> 1 : g; }
-
-  // The step after s (which brings a window) that brings the next one in its run.
-  __device__ static int next_window(const MoeWeight& w, int s) {
-    if (MODE == kOnePerBlock) return (s | 1) + 1;
-    if (MODE == kPowerOfTwo) return (s | ((2 << w.group_shift) - 1)) + 1;
-    return s + w.window;
-  }
-  // Place of step s's first group in the window that step w_s brought, for rows that are row_of(g) modulo 8.
-  __device__ static int index_of(const MoeWeight& w, int s, int w_s, int g, int n_group) {
-    if (MODE == kOnePerBlock) return (s & 1) * 4;
-    if (MODE == kPowerOfTwo) return (s * 4 >> w.group_shift) & 7;
-    const int g0 = group_of(w, w_s * 4);
-    return ((row_of(g) * n_group + g0) & 7) + group_of(w, s * 4) - g0;
-  }
-
-  // Windows of rows row0 + lane / PIECES ..: `at` is the first group of ring row 0's step, counted in the matrix of
-  // `total` groups; rows are n_group apart.
-  template <int ROWS>
-  __device__ static void fetch_window(uint32_t window, int row0, const MoeWeight& w, int64_t at, int n_group,
-                                      int64_t total, int lane) {
-    constexpr int PIECES = kWindowRow / 16;
-#pragma unroll
-    for (int i = 0; i < (ROWS * PIECES + 31) / 32; ++i) {
-      const int row = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
-      if (row >= ROWS) break;
-      const int64_t first = ((at + row * n_group) & ~7ll) + piece * 8;
-      const int bytes = first + 8 <= total ? 16 : first < total ? (int)(total - first) * 2 : 0;
-      const uint32_t dst = window + (row0 + row) * kWindowRow + piece * 16;
-      const int64_t from = bytes ? first : 0;
-      cp_async16(dst, w.scale + from, bytes);
-      if (ASYM) cp_async16(dst + kZeros, w.zp + from, bytes);
+// A round's groups of a row lie in a window of p.window bytes that starts with group window_start of the row: a multiple
+// of eight (counted in the matrix for kAny, where rows start anywhere).
+template <int MODE>
+__device__ __forceinline__ int window_start(const MoeWeight& w, int first_blk) {
+  return MODE == kAny ? group_of(w, first_blk) : group_of(w, first_blk) & ~7;
+}
+// The swizzle that TMA gives a window of 64 or 32 bytes, for rows that are r modulo 8.
+template <int MODE>
+__device__ __forceinline__ int window_swizzle(int bytes, int r) {
+  return MODE == kAny ? 0 : bytes == 64 ? r >> 1 & 3 : bytes == 32 ? r >> 2 & 1 : 0;
+}
+// Copies the windows of `rows` rows (kAny; by the producer warps, a lane per row): row i starts at group at + i * n_group
+// of `total`.
+__device__ __forceinline__ void copy_windows(uint32_t dst, const __half* groups, int rows, int bytes, int64_t at,
+                                             int n_group, int64_t total, int lane) {
+  for (int row = lane; row < rows; row += producers(kAny) * 32) {
+    const int64_t first = (at + row * n_group) & ~7ll;
+    const int left = (int)min((int64_t)bytes, (total - first) * 2);  // what the matrix still holds
+    const __half* src = groups + (left > 0 ? first : 0);
+#pragma unroll 1
+    for (int b = 0; b < bytes; b += 16) {
+      const int n = min(16, max(0, left - b));
+      cp_async16(dst + row * bytes + b, n ? src + b / 2 : src, n);
     }
   }
-};
+}
+
+// Tile row of lane group g: G = 2 reads half pieces, which needs every other pair of rows in a phase.
+template <int G>
+__device__ __forceinline__ int row_of(int g) { return G == 2 ? (g & 1) | (g & 2) << 1 | (g & 4) >> 1 : g; }
 
 __device__ __forceinline__ float half_bits(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)v)); }
 
@@ -334,44 +337,60 @@ struct Sides {
   const uint8_t *m, *f, *s2;
 };
 
-// Adds one step to acc[tile] (rows row_of(g) and + 8 of two tokens, as the mma has them).  `codes` and `window` are the ring's; `index` the place
-// of the step's first group in this lane's row of the window; `operand` this lane's part of the first set in B
-// order, BLOCK bytes from block to block (a lane off the diagonal: zeros); `sides` belong to its two tokens and its
-// block of the first set, MS and FS bytes from block to block.
-template <int G, int R, bool ASYM, int MODE, bool SCALED, int BLOCK, int MS, int FS>
-__device__ __forceinline__ void add_step(float (&acc)[R][4], const uint8_t* codes, const uint8_t* window, int index,
+// Where one step of two 16-row tiles lies: codes of a row 64 bytes apart, TILE bytes from tile to tile; windows of a
+// row `pitch` bytes apart, `window_tile` bytes from tile to tile, zero points `zeros` behind the scales.
+struct StepAt {
+  const uint8_t* codes;
+  const uint8_t* window;
+  int pitch, window_tile, zeros;
+};
+
+// Adds step s to acc[tile] (rows row_of(g) and + 8 of two tokens, as the mma has them).  `start` is the group that the
+// windows start with, `first` the place of that group in this lane's row (kAny); `operand` this lane's part of the
+// first set in B order, BLOCK bytes from block to block (a lane off the diagonal: zeros); `sides` belong to its two
+// tokens and its block of the first set, MS and FS bytes from block to block.
+template <int G, bool ASYM, int MODE, bool SCALED, int TILE, int BLOCK, int MS, int FS>
+__device__ __forceinline__ void add_step(float (&acc)[2][4], const StepAt& at, int start, int first,
                                          const uint8_t* operand, const Sides& sides, int g, int t, int s, int n_blk,
                                          const MoeWeight& w) {
-  using Rg = Ring<G, R, ASYM, MODE>;
-  const int r0 = Rg::row_of(g);
-  const uint8_t* at = window + r0 * Rg::kWindowRow + index * 2;
-  uint2 sc[R][2], zp[ASYM ? R : 1][2];
+  const int r0 = row_of<G>(g), swizzle = window_swizzle<MODE>(at.pitch, r0);
+  const uint8_t* row = at.window + r0 * at.pitch;
+  // place of group x of a row in its window
+  auto place = [&](int x) {
+    const int byte = (x - start + first) * 2;
+    return ((byte >> 4 ^ swizzle) << 4) + (byte & 15);
+  };
+  uint2 sc[2][2], zp[ASYM ? 2 : 1][2];
   if constexpr (MODE == kOnePerBlock) {
+    const uint8_t* from = row + place(s * 4);
 #pragma unroll
-    for (int i = 0; i < 2 * R; ++i) {
-      sc[i / 2][i % 2] = *reinterpret_cast<const uint2*>(at + i * 8 * Rg::kWindowRow);
-      if (ASYM) zp[ASYM ? i / 2 : 0][i % 2] = *reinterpret_cast<const uint2*>(at + i * 8 * Rg::kWindowRow + Rg::kZeros);
-    }
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sc[i][h] = *reinterpret_cast<const uint2*>(from + i * at.window_tile + h * 8 * at.pitch);
+        if (ASYM)
+          zp[ASYM ? i : 0][h] = *reinterpret_cast<const uint2*>(from + i * at.window_tile + h * 8 * at.pitch + at.zeros);
+      }
   }
 #pragma unroll
   for (int j = 0; j < 4 / G; ++j) {
-    // its G words: 16-byte piece (block) of the row, word t mod 4 / G times G
+    // this lane's G words of the set: 16-byte piece (block) of the row, word t mod 4 / G times G
     const int piece = ((j * G + t / (4 / G)) ^ (r0 >> 1 & 3)) * 16 + t % (4 / G) * (4 * G);
-    uint32_t c[2 * R][G];
+    uint32_t c[4][G];
 #pragma unroll
-    for (int i = 0; i < 2 * R; ++i) {
-      const uint8_t* from = codes + (i * 8 + r0) * 64 + piece;
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* from = at.codes + r0 * 64 + piece + i / 2 * TILE + i % 2 * 512;
       if constexpr (G == 4) *reinterpret_cast<uint4*>(c[i]) = *reinterpret_cast<const uint4*>(from);
       else if constexpr (G == 2) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(from);
       else c[i][0] = *reinterpret_cast<const uint32_t*>(from);
     }
     const float4 m = *reinterpret_cast<const float4*>(sides.m + j * G * MS);
-    float d[R][4];
+    float d[2][4];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const uint4 v = *reinterpret_cast<const uint4*>(operand + j * G * BLOCK + i * 16);
 #pragma unroll
-      for (int q = 0; q < R; ++q) {
+      for (int q = 0; q < 2; ++q) {
         uint32_t a[2][4];
         a_operands(c[2 * q][i], c[2 * q + 1][i], a);
         if (i == 0) mma_from(d[q], a[0], v.x, v.y, m);
@@ -385,9 +404,9 @@ __device__ __forceinline__ void add_step(float (&acc)[R][4], const uint8_t* code
     // this lane's block of the set; past the row's last (whose products are zero) the last one's scale will do
     int own = s * 4 + j * G + t / (4 / G);
     if (MODE == kAny) own = min(own, n_blk - 1);
-    const int group = MODE == kOnePerBlock ? 0 : (group_of(w, own) - group_of(w, s * 4)) * 2;
+    const uint8_t* from = MODE == kOnePerBlock ? row : row + place(group_of(w, own));
 #pragma unroll
-    for (int q = 0; q < R; ++q)
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float scale, z = 0.f;
@@ -395,9 +414,9 @@ __device__ __forceinline__ void add_step(float (&acc)[R][4], const uint8_t* code
           scale = group_value<G>(sc[q][h], j, t);
           if (ASYM) z = group_value<G>(zp[ASYM ? q : 0][h], j, t);
         } else {
-          const uint8_t* from = at + (q * 16 + h * 8) * Rg::kWindowRow + group;
-          scale = half_bits(*reinterpret_cast<const uint16_t*>(from));
-          if (ASYM) z = half_bits(*reinterpret_cast<const uint16_t*>(from + Rg::kZeros));
+          const uint8_t* value = from + q * at.window_tile + h * 8 * at.pitch;
+          scale = half_bits(*reinterpret_cast<const uint16_t*>(value));
+          if (ASYM) z = half_bits(*reinterpret_cast<const uint16_t*>(value + at.zeros));
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -424,30 +443,30 @@ __device__ __forceinline__ float block_sum(float v) {
   return v;
 }
 
-// ---- kernel 1: gate / up products, silu, routing weight ------------------------------------------
-constexpr int kUpThreads = 512;  // two 16-row tile pairs (gate, up) x eight slices of K
-constexpr int kUpWarps = kUpThreads / 32;
-constexpr int kUpRows = 32;      // rows of gate and of up per item: one 32-block of h
-constexpr int kUpSlices = 8;
-constexpr int kMaxStages = 4;    // of a ring
+__device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
-// Shared memory of kernel 1 behind the routing: the warps' rings (codes, windows), tokens [NT][4 * steps] blocks of
-// 64 bytes (neighbouring rows in the other half of the banks), their m [NT / 2][blocks + 1] (pairs in different
-// banks) and s2 [NT / 2][blocks], the partial
-// products, 256 bytes of zeros, barriers.
+// ---- kernel 1: gate / up products, silu, routing weight ------------------------------------------
+constexpr int kUpRows = 32;      // rows of gate and of up per item: one 32-block of h
+constexpr int kUpSlices = 8;     // steps of k in a round: a warp takes one, of 16 rows of gate and of up
+constexpr int kUpCodes = kUpSlices * 2 * kUpRows * 64;  // [slice][gate, up][32][64]
+
+// Shared memory of kernel 1 behind the routing: the ring (codes, then windows [scales of gate, of up, zero points of
+// either][32][window]), tokens [NT][4 * steps] blocks of 64 bytes (neighbouring rows in the other half of the banks),
+// their m [NT / 2][blocks + 1] (pairs in different banks) and s2 [NT / 2][blocks], 256 bytes of zeros, barriers.  The
+// partial products of an item [slice][gate, up][NT][32] take the place of the codes of its last round.
 struct UpLayout {
-  int windows, x, row, m, s2, red, zeros, bars, bytes;
-  __host__ __device__ UpLayout(int n_blk, int nt, bool asym, int code_bytes, int window_bytes, int stages) {
+  int windows, window_stage, x, row, m, s2, zeros, bars, bytes;
+  __host__ __device__ UpLayout(int n_blk, int nt, bool asym, int window, int stages) {
     const int blocks = (n_blk + 3) / 4 * 4;
-    windows = kUpWarps * stages * code_bytes;
-    x = windows + kUpWarps * stages * window_bytes;
+    windows = stages * kUpCodes;
+    window_stage = (asym ? 4 : 2) * kUpRows * window;
+    x = windows + stages * window_stage;
     row = blocks * 64 + 64;
     m = x + row * nt;
     s2 = m + nt / 2 * (blocks + 1) * 16;
-    red = s2 + (asym ? nt / 2 * blocks * 8 : 0);
-    zeros = red + kUpSlices * 2 * kUpRows * nt * 4;
+    zeros = s2 + (asym ? nt / 2 * blocks * 8 : 0);
     bars = zeros + 256;
-    bytes = bars + kUpWarps * kMaxStages * 8 + 1024;  // + alignment of the start
+    bytes = bars + 2 * kMaxStages * 8 + 1024;  // + alignment of the start
   }
 };
 
@@ -482,14 +501,13 @@ __device__ __forceinline__ float largest(const uint4& raw) {
 }
 
 struct UpMaps {
-  CUtensorMap gate, up;
+  CUtensorMap codes[2], scale[2], zero[2];  // gate, up
 };
 
 template <int G, bool ASYM, int MODE>
-__global__ void __launch_bounds__(kUpThreads, 1)
-moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int stages) {
-  constexpr int NT = 8 / G;
-  using Rg = Ring<G, 2, ASYM, MODE>;
+__global__ void __launch_bounds__(threads_of(MODE), 1)
+moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
+  constexpr int NT = 8 / G, kStagers = kConsumers * 32, kThreads = threads_of(MODE);
   extern __shared__ uint8_t dyn_raw[];
   uint8_t* dyn = dyn_raw + ((1024u - (sm100::smem_u32(dyn_raw) & 1023u)) & 1023u);
   __shared__ Routing r;
@@ -499,26 +517,79 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int n_blk = p.H / 32, n_steps = (n_blk + 3) / 4, blocks = n_steps * 4;
-  const int n_group = n_blk / p.gate.group_blocks;
-  const UpLayout at(n_blk, NT, ASYM, Rg::kCodes, Rg::kWindow, stages);
-  float* red = reinterpret_cast<float*>(dyn + at.red);  // [slice][gate, up][NT][32]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + at.bars) + warp * kMaxStages;
-  const uint32_t base = sm100::smem_u32(dyn);
+  const int rounds = (n_steps + kUpSlices - 1) / kUpSlices, n_group = n_blk / p.gate.group_blocks;
+  const UpLayout at(n_blk, NT, ASYM, p.window, p.stages);
+  uint64_t* full = reinterpret_cast<uint64_t*>(dyn + at.bars);
+  uint64_t* empty = full + kMaxStages;
   if (tid < 64) reinterpret_cast<uint32_t*>(dyn + at.zeros)[tid] = 0;
   if (tid == 0) {
     abort_flag = 0;
-    sm100::tma_prefetch_desc(&maps.gate);
-    sm100::tma_prefetch_desc(&maps.up);
-  }
-  if (lane == 0) {
-    for (int i = 0; i < stages; ++i) sm100::mbar_init(&bars[i], 1);
+    for (int i = 0; i < p.stages; ++i) {
+      sm100::mbar_init(&full[i], MODE == kAny ? producers(MODE) * 32 + 1 : 1);
+      sm100::mbar_init(&empty[i], kConsumers);
+    }
     sm100::fence_barrier_init();
   }
-  route<NT>(p, r);
+
+  // The tokens whose columns the mma computes: those of the unit at hand, or all of them where they fit.
+  const bool resident = p.T <= NT, bf16 = p.dtype == NPB_BF16, held = blocks * 4 <= kStagers;
+  uint32_t staged = resident ? (p.T < 32 ? (1u << p.T) - 1u : ~0u) : 0u;
+  uint4 raw[NT] = {};
+  auto load = [&](int j) {  // eight elements of each
+    uint32_t m = staged;
+#pragma unroll
+    for (int i = 0; i < NT; ++i, m &= m - 1) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (m != 0 && j < n_blk * 4)
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(p.x) + (int64_t)(__ffs(m) - 1) * (n_blk * 4) + j);
+    }
+  };
+  // Brings the staged tokens to shared memory: the largest magnitude of each, then the stored values; rows of up to
+  // 4096 stay in registers between the two.  (Columns past the last token hold what was there: nothing reads their
+  // sums.)  By the consumers; `loaded` if raw holds them already.
+  auto stage_tokens = [&](bool loaded) {
+    const int n = __popc(staged);
+    if (tid < NT) x_top[tid] = 0;
+    consumer_barrier();  // everybody is through with the tokens before
+    float top[NT] = {};
+#pragma unroll 1
+    for (int j = tid; j < blocks * 4; j += kStagers) {
+      if (!(loaded && held)) load(j);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        top[i] = fmaxf(top[i], bf16 ? largest<__nv_bfloat16>(raw[i]) : largest<__half>(raw[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top[i]));
+      if (lane == 0 && i < n) atomicMax(&x_top[i], bits);
+    }
+    consumer_barrier();
+    if (tid < n) x_f[tid] = power_below(__uint_as_float(x_top[tid]));
+#pragma unroll 1
+    for (int j0 = 0; j0 < blocks * 4; j0 += kStagers) {  // whole warps
+      const int j = j0 + tid;
+      if (!held) load(j);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (i < n) {
+          const float by = 1.f / power_below(__uint_as_float(x_top[i]));
+          uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
+          float* to_m = reinterpret_cast<float*>(dyn + at.m) + (i / 2 * (blocks + 1) + (j >> 2)) * 4 + (i & 1);
+          float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + (i / 2 * blocks + (j >> 2)) * 2 + (i & 1) : nullptr;
+          const bool write = j < blocks * 4;
+          if (bf16) store_operand<__nv_bfloat16>(raw[i], by, to, to_m, to_s2, write, ASYM);
+          else store_operand<__half>(raw[i], by, to, to_m, to_s2, write, ASYM);
+        }
+    }
+    consumer_barrier();
+  };
+  if (resident && held && warp < kConsumers) load(tid);  // on their way while the tokens are routed
+  route<NT>(p, r, reinterpret_cast<uint32_t*>(dyn));
 
   if (blockIdx.x == 0) {  // for kernel 2
     if (tid == 0) p.units->n = r.units.n;
-    for (int i = tid; i < r.units.n; i += kUpThreads) {
+    for (int i = tid; i < r.units.n; i += kThreads) {
       p.units->mask[i] = r.units.mask[i];
       p.units->expert[i] = r.units.expert[i];
       p.units->slot[i] = r.units.slot[i];
@@ -527,206 +598,186 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p, const int 
   const int tiles = p.I / kUpRows;
   const int64_t items = (int64_t)tiles * r.units.n;
   const int first = (int)(items * blockIdx.x / gridDim.x), last = (int)(items * (blockIdx.x + 1) / gridDim.x);
-  const int mt = warp & 1, ks = warp >> 1;
-  const int s_first = n_steps * ks / kUpSlices, s_last = n_steps * (ks + 1) / kUpSlices;
-  const int lane_blk = t / (4 / G);      // this lane's block of a set
-  const bool diag = g / NT == lane_blk;  // it holds the nonzero part of column g
-  const uint8_t* operand = dyn + (diag ? at.x + (g % NT) * at.row + lane_blk * 64 + t % (4 / G) * G * 16 : at.zeros);
-  const int operand_step = diag ? 256 : 0;
-  const int pair = t % (4 / G);
-  const Sides sides{dyn + at.m + (pair * (blocks + 1) + lane_blk) * 16, nullptr,
-                    dyn + at.s2 + (pair * blocks + lane_blk) * 8};
-
-  // the warp's ring runs through its steps of all items
-  const int code_ring = warp * stages * Rg::kCodes, window_ring = at.windows + warp * stages * Rg::kWindow;
-  const int64_t total_groups = (int64_t)p.E * p.I * n_group;
-  int f_item = s_first < s_last ? first : last, f_s = s_first, f_stage = 0, f_window = 0, f_row = 0, f_next = s_first;
-  auto f_start = [&] {
-    if (f_item < last) {
-      const int u = f_item / tiles;
-      f_row = r.units.expert[u] * p.I + (f_item - u * tiles) * kUpRows + mt * 16;
-    }
-  };
-  f_start();
-  auto fetch = [&] {
-    if (f_item < last) {
-      if (lane == 0) {
-        uint8_t* to = dyn + code_ring + f_stage * Rg::kCodes;
-        sm100::mbar_arrive_expect_tx(&bars[f_stage], Rg::kCodes);
-        sm100::tma_load_2d(to, &maps.gate, &bars[f_stage], f_s * 64, f_row);
-        sm100::tma_load_2d(to + 1024, &maps.up, &bars[f_stage], f_s * 64, f_row);
-      }
-      if (f_s == f_next) {
-        f_next = Rg::next_window(p.gate, f_s);
-        const uint32_t to = base + window_ring + f_window * Rg::kWindow;
-        if (++f_window == stages) f_window = 0;
-        const int64_t group = (int64_t)f_row * n_group + group_of(p.gate, f_s * 4);
-        Rg::template fetch_window<16>(to, 0, p.gate, group, n_group, total_groups, lane);
-        Rg::template fetch_window<16>(to, 16, p.up, group, n_group, total_groups, lane);
-      }
-      if (++f_s == s_last) {
-        f_s = f_next = s_first;
-        ++f_item;
-        f_start();
-      }
-      if (++f_stage == stages) f_stage = 0;
-    }
-    cp_async_commit();
-  };
-  for (int i = 0; i < stages; ++i) fetch();
-
-  int unit = -1, n = 0, stage = 0, window = -1;  // of the step at hand
+  int stage = 0;
   uint32_t parity = 0;
+  auto advance = [&] {
+    if (++stage == p.stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  };
   bool ok = true;
-  for (int item = first; item < last; ++item) {
-    const int u = item / tiles, i0 = (item - u * tiles) * kUpRows;
-    const int e = r.units.expert[u];
-    if (u != unit) {
-      if (tid < NT) x_top[tid] = 0;
-      __syncthreads();  // everybody is through with the unit before
-      unit = u;
-      const uint32_t mask = r.units.mask[u];
-      n = __popc(mask);
-      // the unit's tokens, eight elements of each to a thread (columns of an mma past the last token hold what was
-      // there: nothing reads their sums): the largest magnitude of each, then the stored values.  Rows of up to 4096
-      // stay in registers between the two.
-      uint4 raw[NT] = {};
-      auto load = [&](int j) {
-        uint32_t m = mask;
-#pragma unroll
-        for (int i = 0; i < NT; ++i, m &= m - 1) {
-          raw[i] = make_uint4(0, 0, 0, 0);
-          if (i < n && j < n_blk * 4)
-            raw[i] = __ldg(reinterpret_cast<const uint4*>(p.x) + (int64_t)(__ffs(m) - 1) * (n_blk * 4) + j);
+
+  if (warp >= kConsumers) {
+    // ---- producers ----
+    const int thread = tid - kConsumers * 32;
+    const uint32_t base = sm100::smem_u32(dyn);
+    const int64_t total_groups = (int64_t)p.E * p.I * n_group;
+    for (int item = first; item < last && ok; ++item) {
+      const int u = item / tiles, row = r.units.expert[u] * p.I + (item - u * tiles) * kUpRows;
+      for (int round = 0; round < rounds; ++round, advance()) {
+        ok = sm100::mbar_wait_bounded(&empty[stage], parity ^ 1, &abort_flag, p.wait_ns);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
         }
-      };
-      const bool bf16 = p.dtype == NPB_BF16, held = blocks * 4 <= kUpThreads;
-      float top[NT] = {};
+        const int s0 = round * kUpSlices, n = min(kUpSlices, n_steps - s0);
+        const int start = window_start<MODE>(p.gate, s0 * 4);
+        uint8_t* codes = dyn + stage * kUpCodes;
+        const int windows = at.windows + stage * at.window_stage, part = kUpRows * p.window;
+        if (thread == 0) {
+          sm100::mbar_arrive_expect_tx(&full[stage], n * 2 * kUpRows * 64 + (MODE == kAny ? 0 : at.window_stage));
+          for (int i = 0; i < n; ++i)
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+              sm100::tma_load_2d(codes + (i * 2 + w) * kUpRows * 64, &maps.codes[w], &full[stage], (s0 + i) * 64, row);
+          if (MODE != kAny) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              sm100::tma_load_2d(dyn + windows + w * part, &maps.scale[w], &full[stage], start, row);
+              if (ASYM) sm100::tma_load_2d(dyn + windows + (2 + w) * part, &maps.zero[w], &full[stage], start, row);
+            }
+          }
+        }
+        if (MODE == kAny) {
+          const int64_t group = (int64_t)row * n_group + start;
 #pragma unroll 1
-      for (int j = tid; j < blocks * 4; j += kUpThreads) {
-        load(j);
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-          top[i] = fmaxf(top[i], bf16 ? largest<__nv_bfloat16>(raw[i]) : largest<__half>(raw[i]));
+          for (int w = 0; w < (ASYM ? 4 : 2); ++w) {
+            const MoeWeight& from = w & 1 ? p.up : p.gate;
+            copy_windows(base + windows + w * part, w < 2 ? from.scale : from.zp, kUpRows, p.window, group, n_group,
+                         total_groups, thread);
+          }
+          cp_async_arrive(&full[stage]);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top[i]));
-        if (lane == 0 && i < n) atomicMax(&x_top[i], bits);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    // ---- consumers ----
+    const int mt = warp & 1, ks = warp >> 1;
+    const int lane_blk = t / (4 / G);      // this lane's block of a set
+    const bool diag = g / NT == lane_blk;  // it holds the nonzero part of column g
+    const uint8_t* operand = dyn + (diag ? at.x + (g % NT) * at.row + lane_blk * 64 + t % (4 / G) * G * 16 : at.zeros);
+    const int operand_step = diag ? 256 : 0, pair = t % (4 / G);
+    const Sides sides{dyn + at.m + (pair * (blocks + 1) + lane_blk) * 16, nullptr,
+                      dyn + at.s2 + (pair * blocks + lane_blk) * 8};
+    if (resident) stage_tokens(true);
+    for (int item = first; item < last; ++item) {
+      const int u = item / tiles, i0 = (item - u * tiles) * kUpRows, e = r.units.expert[u];
+      const uint32_t mask = r.units.mask[u];
+      if (!resident && mask != staged) {
+        staged = mask;
+        stage_tokens(false);
       }
-      __syncthreads();
-      if (tid < n) x_f[tid] = power_below(__uint_as_float(x_top[tid]));
-#pragma unroll 1
-      for (int j0 = 0; j0 < blocks * 4; j0 += kUpThreads) {  // whole warps
-        const int j = j0 + tid;
-        if (!held) load(j);
+      float acc[2][4] = {};
+      for (int round = 0; round < rounds; ++round) {
+        if (round > 0) advance();
+        const int s = round * kUpSlices + ks;
+        ok = sm100::mbar_wait_bounded(&full[stage], parity, &abort_flag, p.wait_ns) && ok;
+        if (s < n_steps) {
+          const int start = window_start<MODE>(p.gate, round * kUpSlices * 4);
+          const int place = MODE == kAny ? (row_of<G>(g) * n_group + start) & 7 : 0;
+          const uint8_t* windows = dyn + at.windows + stage * at.window_stage;
+          const StepAt here{dyn + stage * kUpCodes + ks * 2 * kUpRows * 64 + mt * 1024, windows + mt * 16 * p.window,
+                            p.window, kUpRows * p.window, 2 * kUpRows * p.window};
+          add_step<G, ASYM, MODE, false, kUpRows * 64, 64, 16, 8>(
+              acc, here, start, place, operand + s * operand_step,
+              Sides{sides.m + s * 64, nullptr, sides.s2 + s * 32}, g, t, s, n_blk, p.gate);
+        }
+        if (round < rounds - 1) {
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&empty[stage]);
+        }
+      }
+      consumer_barrier();  // the last round's codes are read
+      float* red = reinterpret_cast<float*>(dyn + stage * kUpCodes);
+      // the blocks of a set, then the slices of K
+      float* part = red + ks * 2 * NT * kUpRows;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-          if (i < n) {
-            const float by = 1.f / power_below(__uint_as_float(x_top[i]));
-            uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
-            float* to_m = reinterpret_cast<float*>(dyn + at.m) + (i / 2 * (blocks + 1) + (j >> 2)) * 4 + (i & 1);
-            float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + (i / 2 * blocks + (j >> 2)) * 2 + (i & 1) : nullptr;
-            const bool write = j < blocks * 4;
-            if (bf16) store_operand<__nv_bfloat16>(raw[i], by, to, to_m, to_s2, write, ASYM);
-            else store_operand<__half>(raw[i], by, to, to_m, to_s2, write, ASYM);
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float q = block_sum<G>(acc[w][2 * h + c]);
+            if (t < 4 / G) part[(w * NT + 2 * t + c) * kUpRows + mt * 16 + row_of<G>(g) + h * 8] = q;
+          }
+      consumer_barrier();
+      uint32_t m = staged;
+      for (int i = 0; i < warp; ++i) m &= m - 1;
+      const int token = __ffs(m) - 1;  // a warp per column, a lane per row
+      if (warp < NT && token >= 0 && (mask >> token & 1)) {
+        float gate = 0.f, up = 0.f;
+#pragma unroll
+        for (int k = 0; k < kUpSlices; ++k) {
+          const float* from = red + (k * 2 * NT + warp) * kUpRows + lane;
+          gate += from[0];
+          up += from[NT * kUpRows];
+        }
+        gate *= x_f[warp];
+        up *= x_f[warp];
+        const bool chosen = lane < p.top_k && r.id[token][lane] == e;
+        const int j = __ffs(__ballot_sync(0xffffffffu, chosen)) - 1;
+        const float h = r.weight[token][j] * (gate / (1.f + expf(-gate)) * up);
+        // the power of two at or below the block's largest magnitude (1 for a block of zeros or with inf / NaN)
+        const float f = power_below(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h)))));
+        const bool is_odd = lane & 1;  // pair (lane & 3) of its word
+        const __half v = __float2half_rn(h * ((is_odd ? 0.0625f : 1.f) / f));
+        const float even = warp_sum(is_odd ? 0.f : __half2float(v)), odd = warp_sum(is_odd ? __half2float(v) : 0.f);
+        const int rank = __popc(mask & ((1u << token) - 1u)), side = rank & 1;
+        const int padded = (tiles + 3) / 4 * 4;
+        uint8_t* rec = p.h + ((int64_t)(r.units.slot[u] + rank / 2) * padded + i0 / 32) * kRecord;
+        reinterpret_cast<__half*>(rec)[side * 32 + (lane & 24) + (lane & 3) * 2 + ((lane >> 2) & 1)] = v;
+        if (lane == 0) {
+          float* to = reinterpret_cast<float*>(rec + 128) + side;
+          put_sides(to, to + 6, even, odd, p.down.zp != nullptr);
+          to[4] = f;
+        }
+        if (i0 / 32 == tiles - 1)  // zeros behind the last block, up to a whole step
+          for (int i = tiles; i < padded; ++i) {
+            rec += kRecord;
+            reinterpret_cast<__half*>(rec)[side * 32 + lane] = __ushort_as_half(0);
+            if (lane < 4) reinterpret_cast<float*>(rec + 128)[side + lane * 2] = 0.f;
           }
       }
-      __syncthreads();
-    }
-    float acc[2][4] = {};
-    int w_s = 0, w_next = s_first;
-    for (int s = s_first; s < s_last; ++s) {
-      ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
-      cp_async_wait(stages - 1);
+      sm100::fence_proxy_async_smem();  // TMA writes there next
       __syncwarp();
-      if (s == w_next) {
-        if (++window == stages) window = 0;
-        w_s = s;
-        w_next = Rg::next_window(p.gate, s);
-      }
-      const int index = Rg::index_of(p.gate, s, w_s, g, n_group);
-      const Sides here{sides.m + s * 64, nullptr, sides.s2 + s * 32};
-      add_step<G, 2, ASYM, MODE, false, 64, 16, 8>(acc, dyn + code_ring + stage * Rg::kCodes,
-                                               dyn + window_ring + window * Rg::kWindow, index, operand + s * operand_step, here, g, t, s, n_blk, p.gate);
-      __syncwarp();
-      fetch();
-      if (++stage == stages) { stage = 0; parity ^= 1; }
-    }
-    __syncthreads();  // the item before is read
-    // the blocks of a set, then the slices of K
-    float* part = red + ks * 2 * NT * kUpRows;
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float q = block_sum<G>(acc[w][2 * h + c]);
-          if (t < 4 / G) part[(w * NT + 2 * t + c) * kUpRows + mt * 16 + Rg::row_of(g) + h * 8] = q;
-        }
-      }
-    __syncthreads();
-    if (warp < n) {  // a warp per token, a lane per row
-      float gate = 0.f, up = 0.f;
-#pragma unroll
-      for (int k = 0; k < kUpSlices; ++k) {
-        const float* from = red + (k * 2 * NT + warp) * kUpRows + lane;
-        gate += from[0];
-        up += from[NT * kUpRows];
-      }
-      gate *= x_f[warp];
-      up *= x_f[warp];
-      uint32_t m = r.units.mask[u];
-      for (int i = 0; i < warp; ++i) m &= m - 1;
-      const int token = __ffs(m) - 1;
-      float weight = 0.f;
-      for (int j = 0; j < p.top_k; ++j)
-        if (r.id[token][j] == e) weight = r.weight[token][j];
-      const float h = weight * (gate / (1.f + expf(-gate)) * up);
-      float top = fabsf(h);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float f = power_below(top);
-      const bool is_odd = lane & 1;  // pair (lane & 3) of its word
-      const __half v = __float2half_rn(h * ((is_odd ? 0.0625f : 1.f) / f));
-      const float even = warp_sum(is_odd ? 0.f : __half2float(v)), odd = warp_sum(is_odd ? __half2float(v) : 0.f);
-      uint8_t* rec = p.h + ((int64_t)(r.units.slot[u] + warp / 2) * (p.I / 32) + i0 / 32) * kRecord;
-      reinterpret_cast<__half*>(rec)[(warp & 1) * 32 + (lane & 24) + (lane & 3) * 2 + ((lane >> 2) & 1)] = v;
-      if (lane == 0) {
-        float* to = reinterpret_cast<float*>(rec + 128) + (warp & 1);
-        put_sides(to, to + 6, even, odd, p.down.zp != nullptr);
-        to[4] = f;
-      }
+      if (lane == 0) sm100::mbar_arrive(&empty[stage]);
+      advance();
     }
   }
-  if (!ok) atomicExch(&g_moe_status, 1);
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  if (!ok) {  // let copies that were issued land before the shared memory is released
-    const uint64_t t0 = sm100::global_timer_ns();
+  if (!ok) {
+    atomicExch(&g_moe_status, 1);
+    const uint64_t t0 = sm100::global_timer_ns();  // let copies that were issued land
     while (sm100::global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
 }
 
 // ---- kernel 2: down product and the sum over experts ----------------------------------------------
-constexpr int kDownThreads = 256;
-constexpr int kDownWarps = kDownThreads / 32;
-constexpr int kDownTiles = 4;                 // 16-row tiles per warp: h is brought once for all of them
-constexpr int kDownRows = 16 * kDownTiles;    // output rows per cluster
-constexpr int kDownSplit = 4;                 // CTAs of a cluster: each takes a share of the (unit, step) sequence
-
-// Shared memory of kernel 2 behind the routing: per warp a ring of codes, a ring of windows and h records
-// [NT / 2][4], the partial sums [T][64]; then zeros that cover the reach of a step's operands, barriers.
+// A CTA has 512 / slices rows of the output, 32 to each of 16 / slices warps side by side, and takes a share of the
+// (unit, round) pairs of its cluster.
+// Shared memory of kernel 2 behind the lists: the ring (codes [slice][rows][64], then windows [scales, zero points]
+// [rows][window], then h records [NT / 2][4 * slices], pairs in different banks), the sums [T][rows], zeros that
+// cover the reach of a step's operands, barriers.  The partial products of a unit [slice][NT][rows] take the place of the codes
+// of its last round.
 struct DownLayout {
-  int rest, stage, windows, warp_rest, zeros, bars, bytes;
-  __host__ __device__ DownLayout(int T, int nt, int code_bytes, int window_bytes, int stages) {
-    rest = kDownWarps * stages * code_bytes;
-    stage = window_bytes + nt / 2 * 4 * kRecord;
-    warp_rest = stages * stage + T * kDownRows * 4;
-    zeros = rest + kDownWarps * warp_rest;
+  int rows, windows, window_stage, h, h_pair, h_stage, sums, zeros, bars, bytes;
+  __host__ __device__ DownLayout(int T, int nt, bool asym, int window, int slices, int stages) {
+    rows = 512 / slices;
+    windows = stages * 512 * 64;
+    window_stage = (asym ? 2 : 1) * rows * window;
+    h = windows + stages * window_stage;
+    h_pair = 4 * slices * kRecord + 32;
+    h_stage = nt / 2 * h_pair;
+    sums = h + stages * h_stage;
+    zeros = sums + T * rows * 4;
     bars = zeros + 4 * kRecord;
-    bytes = bars + kDownWarps * kMaxStages * 8 + 1024;
+    bytes = bars + 2 * kMaxStages * 8 + 1024;
   }
+};
+
+struct DownMaps {
+  CUtensorMap codes, scale, zero;
 };
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
@@ -736,198 +787,181 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 }
 
 template <int G, bool ASYM, int MODE>
-__global__ void __cluster_dims__(kDownSplit, 1, 1) __launch_bounds__(kDownThreads, G == 1 ? 1 : 2)
-moe_down_kernel(const __grid_constant__ CUtensorMap map, const MoeParams p, const int stages) {
-  constexpr int NT = 8 / G;
-  using Rg = Ring<G, kDownTiles, ASYM, MODE>;
+__global__ void __launch_bounds__(threads_of(MODE), 1)
+moe_down_kernel(const __grid_constant__ DownMaps maps, const MoeParams p) {
+  constexpr int NT = 8 / G, kThreads = threads_of(MODE);
   extern __shared__ uint8_t dyn_raw[];
   uint8_t* dyn = dyn_raw + ((1024u - (sm100::smem_u32(dyn_raw) & 1023u)) & 1023u);
-  __shared__ Units u;
+  __shared__ Units lists;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int n_blk = p.I / 32, n_steps = (n_blk + 3) / 4, n_group = n_blk / p.down.group_blocks;
-  const int rank = (int)sm100::cluster_ctarank();
-  const int j0 = blockIdx.x / kDownSplit * kDownRows;
-  const int rows_left = min(kDownRows, p.H - j0);  // 32 in the last cluster of an odd H / 32
-  const DownLayout at(p.T, NT, Rg::kCodes, Rg::kWindow, stages);
-  const uint32_t base = sm100::smem_u32(dyn);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + at.bars) + warp * kMaxStages;
-  const int code_ring = warp * stages * Rg::kCodes, rest_ring = at.rest + warp * at.warp_rest;
-  auto sums_of = [&](int w) {
-    return reinterpret_cast<float*>(dyn + at.rest + w * at.warp_rest + stages * at.stage);  // [T][64]
-  };
-  float* sums = sums_of(warp);
-  for (int i = lane; i < p.T * kDownRows; i += 32) sums[i] = 0.f;
-  for (int i = tid; i < kRecord; i += kDownThreads) reinterpret_cast<uint32_t*>(dyn + at.zeros)[i] = 0;
+  const int rounds = (n_steps + p.slices - 1) / p.slices;
+  const int rank = p.split > 1 ? (int)sm100::cluster_ctarank() : 0;
+  const DownLayout at(p.T, NT, ASYM, p.window, p.slices, p.stages);
+  const int rows = at.rows, j0 = blockIdx.x / p.split * rows, rows_left = min(rows, p.H - j0);
+  float* sums = reinterpret_cast<float*>(dyn + at.sums);
+  uint64_t* full = reinterpret_cast<uint64_t*>(dyn + at.bars);
+  uint64_t* empty = full + kMaxStages;
+  for (int i = tid; i < p.T * rows; i += kThreads) sums[i] = 0.f;
+  for (int i = tid; i < kRecord; i += kThreads) reinterpret_cast<uint32_t*>(dyn + at.zeros)[i] = 0;
   if (tid == 0) {
     abort_flag = 0;
-    sm100::tma_prefetch_desc(&map);
-  }
-  if (lane == 0) {
-    for (int i = 0; i < stages; ++i) sm100::mbar_init(&bars[i], 1);
+    for (int i = 0; i < p.stages; ++i) {
+      sm100::mbar_init(&full[i], MODE == kAny ? producers(MODE) * 32 + 1 : 1);
+      sm100::mbar_init(&empty[i], kConsumers);
+    }
     sm100::fence_barrier_init();
   }
   const int n_units = __ldcg(&p.units->n);
-  for (int i = tid; i < n_units; i += kDownThreads) {
-    u.mask[i] = __ldcg(&p.units->mask[i]);
-    u.expert[i] = __ldcg(&p.units->expert[i]);
-    u.slot[i] = __ldcg(&p.units->slot[i]);
+  for (int i = tid; i < n_units; i += kThreads) {
+    lists.mask[i] = __ldcg(&p.units->mask[i]);
+    lists.expert[i] = __ldcg(&p.units->expert[i]);
+    lists.slot[i] = __ldcg(&p.units->slot[i]);
   }
   __syncthreads();
 
-  // (unit, step) pairs in a row, an equal share of consecutive ones per warp of the cluster
-  const int64_t total = (int64_t)n_units * n_steps;
-  const int share = rank * kDownWarps + warp, shares = kDownSplit * kDownWarps;
-  const int first = (int)(total * share / shares), last = (int)(total * (share + 1) / shares);
-  const int lane_blk = t / (4 / G);
-  const bool diag = g / NT == lane_blk;
-  const uint8_t* operand = dyn + (diag ? rest_ring + Rg::kWindow + (g % NT / 2 * 4 + lane_blk) * kRecord + (g & 1) * 64 +
-                                             t % (4 / G) * G * 16
-                                       : at.zeros);
-  const int operand_stage = diag ? at.stage : 0;
-  const uint8_t* sides = dyn + rest_ring + Rg::kWindow + (t % (4 / G) * 4 + lane_blk) * kRecord + 128;
-
-  const int64_t total_groups = (int64_t)p.E * p.H * n_group;
-  const int first_u = first / n_steps, first_s = first - first_u * n_steps;
-  // a run of windows is what the warp does of one unit
-  int f_at = first, f_u = first_u, f_s = first_s, f_stage = 0, f_window = 0, f_next = first_s;
-  auto fetch_weights = [&] {
-    const int row0 = u.expert[f_u] * p.H + j0;
-    if (lane == 0) {
-      sm100::mbar_arrive_expect_tx(&bars[f_stage], Rg::kCodes);
-      sm100::tma_load_2d(dyn + code_ring + f_stage * Rg::kCodes, &map, &bars[f_stage], f_s * 64, row0);
-    }
-    if (f_s == f_next) {
-      f_next = Rg::next_window(p.down, f_s);
-      Rg::template fetch_window<kDownRows>(base + rest_ring + f_window * at.stage, 0, p.down,
-                                           (int64_t)row0 * n_group + group_of(p.down, f_s * 4), n_group, total_groups,
-                                           lane);
-      if (++f_window == stages) f_window = 0;
-    }
-  };
-  constexpr int kPieces = kRecord / 16, kParts = (NT / 2 * 4 * kPieces + 31) / 32;
-  int part_src[kParts];  // of this lane's 16-byte pieces of a step's records, from the unit's first of the step on
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) {
-    const int c = i * 32 + lane, pair = c / (4 * kPieces);
-    part_src[i] = pair * n_blk * kRecord + (c - pair * 4 * kPieces) * 16;
-  }
-  auto fetch_records = [&] {  // blocks 4 f_s .. + 4 of the unit's tokens; zeros past n_blk
-    const uint8_t* rec = p.h + ((int64_t)u.slot[f_u] * n_blk + f_s * 4) * kRecord;
-    const int pieces = (__popc(u.mask[f_u]) + 1) / 2 * 4 * kPieces;
-    const uint32_t to = base + rest_ring + f_stage * at.stage + Rg::kWindow + lane * 16;
-    const int whole = (n_blk - f_s * 4) * kPieces;  // pieces of a pair that exist
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const int c = i * 32 + lane;
-      const bool valid = MODE != kAny || c % (4 * kPieces) < whole;
-      if (c < pieces) cp_async16(to + i * 512, valid ? rec + part_src[i] : p.h, valid ? 16 : 0);
-    }
-  };
-  auto advance = [&] {
-    cp_async_commit();
-    if (f_at < last) {
-      ++f_at;
-      if (++f_s == n_steps) {
-        f_s = f_next = 0;
-        ++f_u;
-      }
-      if (++f_stage == stages) f_stage = 0;
-    }
-  };
-
-  float acc[kDownTiles][4] = {};
-  int unit = -1;
-  auto flush = [&] {
-    uint32_t m = unit >= 0 ? u.mask[unit] : 0u;
-    for (int i = 0; i < 2 * t; ++i) m &= m - 1;  // of this lane's two tokens
-    const int token[2] = {__ffs(m) - 1, __ffs(m & (m - 1)) - 1};
-#pragma unroll
-    for (int w = 0; w < kDownTiles; ++w)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float q = block_sum<G>(acc[w][2 * h + c]);
-          if (t < 4 / G && token[c] >= 0) sums[token[c] * kDownRows + w * 16 + h * 8 + Rg::row_of(g)] += q;
-          acc[w][2 * h + c] = 0.f;
-        }
-      }
-    __syncwarp();
-  };
-
-  int c_u = first_u, c_s = first_s, stage = 0, window = -1, w_s = 0, w_next = first_s;
+  const int64_t total = (int64_t)n_units * rounds;
+  const int first = (int)(total * rank / p.split), last = (int)(total * (rank + 1) / p.split);
+  const int first_u = first / rounds;
+  int u = first_u, round = first - first_u * rounds;  // of the pair at hand
+  int stage = 0;
   uint32_t parity = 0;
+  auto advance = [&] {
+    if (++round == rounds) {
+      round = 0;
+      ++u;
+    }
+    if (++stage == p.stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  };
   bool ok = true;
-  for (int q = first - stages; q < last; ++q) {
-    if (q >= first) {
-      if (c_u != unit) {
-        flush();
-        unit = c_u;
+
+  if (warp >= kConsumers) {
+    // ---- producers ----
+    const int thread = tid - kConsumers * 32;
+    const uint32_t base = sm100::smem_u32(dyn);
+    const int64_t total_groups = (int64_t)p.E * p.H * n_group;
+    for (int q = first; q < last; ++q, advance()) {
+      ok = sm100::mbar_wait_bounded(&empty[stage], parity ^ 1, &abort_flag, p.wait_ns);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
       }
-      ok = sm100::mbar_wait_bounded(&bars[stage], parity, &abort_flag, p.wait_ns) && ok;
-      cp_async_wait(stages - 1);
-      __syncwarp();
-      if (c_s == w_next) {
-        if (++window == stages) window = 0;
-        w_s = c_s;
-        w_next = Rg::next_window(p.down, c_s);
+      const int row = lists.expert[u] * p.H + j0, s0 = round * p.slices, n = min(p.slices, n_steps - s0);
+      const int start = window_start<MODE>(p.down, s0 * 4), pairs = (__popc(lists.mask[u]) + 1) / 2;
+      const int windows = at.windows + stage * at.window_stage, part = rows * p.window;
+      const uint32_t h_bytes = n * 4 * kRecord;
+      if (thread == 0) {
+        sm100::mbar_arrive_expect_tx(&full[stage], n * rows * 64 + pairs * h_bytes + (MODE == kAny ? 0 : at.window_stage));
+        for (int i = 0; i < n; ++i)
+          sm100::tma_load_2d(dyn + stage * 512 * 64 + i * rows * 64, &maps.codes, &full[stage], (s0 + i) * 64, row);
+        if (MODE != kAny) {
+          sm100::tma_load_2d(dyn + windows, &maps.scale, &full[stage], start, row);
+          if (ASYM) sm100::tma_load_2d(dyn + windows + part, &maps.zero, &full[stage], start, row);
+        }
+        for (int i = 0; i < pairs; ++i)
+          bulk_load(base + at.h + stage * at.h_stage + i * at.h_pair,
+                    p.h + ((int64_t)(lists.slot[u] + i) * (n_steps * 4) + s0 * 4) * kRecord, h_bytes, &full[stage]);
       }
-      const int index = Rg::index_of(p.down, c_s, w_s, g, n_group);
-      const uint8_t* side = sides + stage * at.stage;
-      add_step<G, kDownTiles, ASYM, MODE, true, kRecord, kRecord, kRecord>(acc, dyn + code_ring + stage * Rg::kCodes,
-                                                                  dyn + rest_ring + window * at.stage, index, operand + stage * operand_stage,
-                                                                  Sides{side, side + 16, side + 24}, g, t, c_s, n_blk,
-                                                                  p.down);
-      __syncwarp();
-      if (++c_s == n_steps) {
-        c_s = w_next = 0;
-        ++c_u;
-      }
-      if (++stage == stages) {
-        stage = 0;
-        parity ^= 1;
+      if (MODE == kAny) {
+        const int64_t group = (int64_t)row * n_group + start;
+        copy_windows(base + windows, p.down.scale, rows, p.window, group, n_group, total_groups, thread);
+        if (ASYM) copy_windows(base + windows + part, p.down.zp, rows, p.window, group, n_group, total_groups, thread);
+        cp_async_arrive(&full[stage]);
       }
     }
-    if (f_at < last) {
-      fetch_weights();
-      fetch_records();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    // ---- consumers ----
+    const int ks = warp % p.slices, r0 = warp / p.slices * 32;  // slice of a round, rows of the CTA's
+    const int lane_blk = t / (4 / G);
+    const bool diag = g / NT == lane_blk;
+    const uint8_t* operand = dyn + (diag ? at.h + g % NT / 2 * at.h_pair + (ks * 4 + lane_blk) * kRecord + (g & 1) * 64 +
+                                               t % (4 / G) * G * 16
+                                         : at.zeros);
+    const int operand_stage = diag ? at.h_stage : 0;
+    const uint8_t* sides = dyn + at.h + t % (4 / G) * at.h_pair + (ks * 4 + lane_blk) * kRecord + 128;
+    float acc[2][4] = {};
+    for (int q = first; q < last; ++q, advance()) {
+      const int s = round * p.slices + ks;
+      ok = sm100::mbar_wait_bounded(&full[stage], parity, &abort_flag, p.wait_ns) && ok;
+      if (s < n_steps) {
+        const int start = window_start<MODE>(p.down, round * p.slices * 4);
+        const int place = MODE == kAny ? (row_of<G>(g) * n_group + start) & 7 : 0;
+        const StepAt here{dyn + stage * 512 * 64 + (ks * rows + r0) * 64,
+                          dyn + at.windows + stage * at.window_stage + r0 * p.window, p.window, 16 * p.window,
+                          rows * p.window};
+        const uint8_t* side = sides + stage * at.h_stage;
+        add_step<G, ASYM, MODE, true, 1024, kRecord, kRecord, kRecord>(
+            acc, here, start, place, operand + stage * operand_stage, Sides{side, side + 16, side + 24}, g, t, s, n_blk,
+            p.down);
+      }
+      if (round == rounds - 1 || q == last - 1) {
+        // the unit (or this CTA's share of it) is done: its slices of k, and its tokens into the sums
+        consumer_barrier();  // the round's codes are read
+        float* red = reinterpret_cast<float*>(dyn + stage * 512 * 64);
+        float* part = red + ks * NT * rows + r0;
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float v = block_sum<G>(acc[w][2 * h + c]);
+              if (t < 4 / G) part[(2 * t + c) * rows + w * 16 + h * 8 + row_of<G>(g)] = v;
+              acc[w][2 * h + c] = 0.f;
+            }
+        consumer_barrier();
+        const uint32_t mask = lists.mask[u];
+        const int n = __popc(mask);
+        for (int i = tid; i < n * rows; i += kConsumers * 32) {
+          const int c = i / rows, row = i - c * rows;
+          uint32_t m = mask;
+          for (int k = 0; k < c; ++k) m &= m - 1;
+          float v = 0.f;
+          for (int k = 0; k < p.slices; ++k) v += red[(k * NT + c) * rows + row];
+          sums[(__ffs(m) - 1) * rows + row] += v;
+        }
+        sm100::fence_proxy_async_smem();  // TMA writes there next
+      }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&empty[stage]);
     }
-    advance();
   }
-  flush();
-  asm volatile("cp.async.wait_all;" ::: "memory");
   if (!ok) {
     atomicExch(&g_moe_status, 2);
     const uint64_t t0 = sm100::global_timer_ns();
     while (sm100::global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
   __syncthreads();
-  // the warps of the CTA (into warp 0's sums), then the CTAs of the cluster: each finishes a quarter of the rows
-  float* cta_sums = sums_of(0);
-  for (int i = tid; i < p.T * kDownRows; i += kDownThreads) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDownWarps; ++w) v += sums_of(w)[i];
-    cta_sums[i] = v;
+  // the CTAs of the cluster: each finishes an equal share of the rows
+  if (p.split > 1) {
+    __syncwarp();
+    sm100::cluster_sync_all();
   }
-  __syncwarp();
-  sm100::cluster_sync_all();
-  constexpr int kRowsEach = kDownRows / kDownSplit;
-  for (int i = tid; i < p.T * kRowsEach; i += kDownThreads) {
-    const int token = i / kRowsEach, row = rank * kRowsEach + i % kRowsEach;
+  const int each = rows / p.split;
+  for (int i = tid; i < p.T * each; i += kThreads) {
+    const int token = i / each, row = rank * each + i % each;
     float v = 0.f;
-#pragma unroll
-    for (int c = 0; c < kDownSplit; ++c)
-      v += ld_cluster_f32(sm100::map_to_cta(sm100::smem_u32(cta_sums) + (token * kDownRows + row) * 4, c));
+    if (p.split > 1) {
+      for (int c = 0; c < p.split; ++c)
+        v += ld_cluster_f32(sm100::map_to_cta(sm100::smem_u32(sums) + (token * rows + row) * 4, c));
+    } else {
+      v = sums[token * rows + row];
+    }
     if (row >= rows_left) continue;
     const int64_t to = (int64_t)token * p.H + j0 + row;
     if (p.dtype == NPB_BF16) static_cast<__nv_bfloat16*>(p.y)[to] = from_f32<__nv_bfloat16>(v);
     else static_cast<__half*>(p.y)[to] = from_f32<__half>(v);
   }
-  __syncwarp();
-  sm100::cluster_sync_all();  // nobody leaves while its sums are read
+  if (p.split > 1) {
+    __syncwarp();
+    sm100::cluster_sync_all();  // nobody leaves while its sums are read
+  }
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -936,67 +970,111 @@ int mode_of(const MoeWeight& w, int n_blk) {
   return w.group_blocks == 1 ? kOnePerBlock : kPowerOfTwo;
 }
 
-// Codes [rows, bytes of a row] in boxes of 64 bytes x box_rows.
+// Bytes of a row's groups in a round of `slices` steps.
+int window_bytes(const MoeWeight& w, int n_blk, int slices) {
+  const int blocks = 4 * slices, gb = w.group_blocks;
+  switch (mode_of(w, n_blk)) {
+    case kOnePerBlock: return blocks * 2;
+    case kPowerOfTwo: return blocks * 2 / gb > 16 ? blocks * 2 / gb : 16;
+    default:  // the groups that `blocks` blocks touch, behind up to seven others
+      return (((blocks - 1 + gb - 1) / gb + 1 + 7) * 2 + 15) / 16 * 16;
+  }
+}
+
+// Codes [rows, bytes of a row] in boxes of 64 bytes x box_rows, and groups [rows, n_group] in boxes of a window.
 int make_code_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int64_t row_bytes, int box_rows) {
   return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, row_bytes, box_rows, 64,
                             CU_TENSOR_MAP_SWIZZLE_64B);
 }
+int make_group_map(CUtensorMap* map, const __half* groups, int64_t rows, int64_t n_group, int box_rows, int window) {
+  return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, groups, rows, n_group, box_rows, window / 2,
+                            window == 64   ? CU_TENSOR_MAP_SWIZZLE_64B
+                            : window == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                           : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
 
 // Ring stages that fit next to the rest (2..4; 0: not even two do).
 template <typename Bytes>
-int pick_stages(Bytes bytes, int static_bytes, int ctas_per_sm) {
-  const int cap = ctas_per_sm == 1 ? max_dynamic_smem() : (max_dynamic_smem() - 1024) / ctas_per_sm - 1024;
+int pick_stages(Bytes bytes, int static_bytes) {
   int stages = kMaxStages;
-  while (stages >= 2 && bytes(stages) + static_bytes > cap) --stages;
+  while (stages >= 2 && bytes(stages) + static_bytes > max_dynamic_smem()) --stages;
   return stages >= 2 ? stages : 0;
 }
 
-int window_bytes(int rows, bool asym, int mode) { return rows * (mode == kAny ? 32 : 16) * (asym ? 2 : 1); }
-
-int up_bytes(const MoeParams& p, int g, int stages) {
-  return UpLayout(p.H / 32, 8 / g, p.gate.zp != nullptr, 32 * 64,
-                  window_bytes(32, p.gate.zp != nullptr, mode_of(p.gate, p.H / 32)), stages).bytes;
+// Fills in the ring of a kernel; false: it does not fit.
+bool plan_up(MoeParams& p, int g) {
+  p.window = window_bytes(p.gate, p.H / 32, kUpSlices);
+  p.stages = pick_stages(
+      [&](int n) { return UpLayout(p.H / 32, 8 / g, p.gate.zp != nullptr, p.window, n).bytes; }, (int)sizeof(Routing) + 128);
+  return p.stages != 0;
 }
-int up_stages(const MoeParams& p, int g) {
-  return pick_stages([&](int n) { return up_bytes(p, g, n); }, (int)sizeof(Routing) + 256, 1);
-}
-int down_bytes(const MoeParams& p, int g, int stages) {
-  return DownLayout(p.T, 8 / g, kDownRows * 64,
-                    window_bytes(kDownRows, p.down.zp != nullptr, mode_of(p.down, p.I / 32)), stages).bytes;
-}
-int down_stages(const MoeParams& p, int g) {
-  auto bytes = [&](int n) { return down_bytes(p, g, n); };
-  const int two = g == 1 ? 0 : pick_stages(bytes, (int)sizeof(Units) + 256, 2);  // two CTAs on an SM where they fit
-  return two ? two : pick_stages(bytes, (int)sizeof(Units) + 256, 1);
+bool plan_down(MoeParams& p, int g) {
+  // 128 rows to a CTA and a cluster of up to four, as long as that makes a CTA for most SMs; fewer rows otherwise
+  p.slices = p.H >= 4096 ? 4 : p.H >= 2048 ? 8 : 16;
+  const int rows = 512 / p.slices, tiles = (p.H + rows - 1) / rows;
+  p.split = 1;
+  while (p.split < 4 && tiles * p.split * 2 <= sm_count()) p.split *= 2;
+  p.window = window_bytes(p.down, p.I / 32, p.slices);
+  p.stages = pick_stages(
+      [&](int n) { return DownLayout(p.T, 8 / g, p.down.zp != nullptr, p.window, p.slices, n).bytes; },
+      (int)sizeof(Units) + 512);
+  return p.stages != 0;
 }
 
 template <int G, bool ASYM, int MODE>
-int launch_up(const MoeParams& p, cudaStream_t st) {
+int launch_up(MoeParams p, cudaStream_t st) {
   auto kern = moe_up_kernel<G, ASYM, MODE>;
-  const int stages = up_stages(p, G), smem = up_bytes(p, G, stages);
+  if (!plan_up(p, G)) return NPB_ERR_TOO_LARGE;
+  const int n_blk = p.H / 32, smem = UpLayout(n_blk, 8 / G, ASYM, p.window, p.stages).bytes;
   int per_sm = 0;
-  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kUpThreads, smem, &per_sm)) return rc;
+  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), threads_of(MODE), smem, &per_sm)) return rc;
   if (per_sm < 1) return NPB_ERR_TOO_LARGE;
-  UpMaps maps;
-  if (int rc = make_code_map(&maps.gate, p.gate.codes, (int64_t)p.E * p.I, p.H / 2, 16)) return rc;
-  if (int rc = make_code_map(&maps.up, p.up.codes, (int64_t)p.E * p.I, p.H / 2, 16)) return rc;
+  UpMaps maps{};
+  const int64_t rows = (int64_t)p.E * p.I, n_group = n_blk / p.gate.group_blocks;
+  const MoeWeight* w[2] = {&p.gate, &p.up};
+  for (int i = 0; i < 2; ++i) {
+    if (int rc = make_code_map(&maps.codes[i], w[i]->codes, rows, p.H / 2, kUpRows)) return rc;
+    if (MODE == kAny) continue;
+    if (int rc = make_group_map(&maps.scale[i], w[i]->scale, rows, n_group, kUpRows, p.window)) return rc;
+    if (!ASYM) continue;
+    if (int rc = make_group_map(&maps.zero[i], w[i]->zp, rows, n_group, kUpRows, p.window)) return rc;
+  }
   const int64_t active = p.T * p.top_k < p.E ? p.T * p.top_k : p.E;
   const int64_t most = active * (p.I / kUpRows), slots = (int64_t)sm_count() * per_sm;
-  kern<<<(unsigned)(most < slots ? most : slots), kUpThreads, smem, st>>>(maps, p, stages);
+  kern<<<(unsigned)(most < slots ? most : slots), threads_of(MODE), smem, st>>>(maps, p);
   NPB_LAUNCH_CHECK();
   return NPB_OK;
 }
 
 template <int G, bool ASYM, int MODE>
-int launch_down(const MoeParams& p, cudaStream_t st) {
+int launch_down(MoeParams p, cudaStream_t st) {
   auto kern = moe_down_kernel<G, ASYM, MODE>;
-  const int stages = down_stages(p, G), smem = down_bytes(p, G, stages);
+  if (!plan_down(p, G)) return NPB_ERR_TOO_LARGE;
+  const DownLayout at(p.T, 8 / G, ASYM, p.window, p.slices, p.stages);
   int per_sm = 0;
-  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kDownThreads, smem, &per_sm)) return rc;
+  if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), threads_of(MODE), at.bytes, &per_sm)) return rc;
   if (per_sm < 1) return NPB_ERR_TOO_LARGE;
-  CUtensorMap map;
-  if (int rc = make_code_map(&map, p.down.codes, (int64_t)p.E * p.H, p.I / 2, kDownRows)) return rc;
-  kern<<<(unsigned)((p.H + kDownRows - 1) / kDownRows * kDownSplit), kDownThreads, smem, st>>>(map, p, stages);
+  DownMaps maps{};
+  const int64_t rows = (int64_t)p.E * p.H, n_group = p.I / 32 / p.down.group_blocks;
+  if (int rc = make_code_map(&maps.codes, p.down.codes, rows, p.I / 2, at.rows)) return rc;
+  if (MODE != kAny) {
+    if (int rc = make_group_map(&maps.scale, p.down.scale, rows, n_group, at.rows, p.window)) return rc;
+    if (ASYM)
+      if (int rc = make_group_map(&maps.zero, p.down.zp, rows, n_group, at.rows, p.window)) return rc;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((p.H + at.rows - 1) / at.rows * p.split));
+  cfg.blockDim = dim3(threads_of(MODE));
+  cfg.dynamicSmemBytes = at.bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.split;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, p));
   NPB_LAUNCH_CHECK();
   return NPB_OK;
 }
@@ -1025,7 +1103,10 @@ int launch(const MoeParams& p, cudaStream_t st) {
 
 int launch_tokens(const MoeParams& p, cudaStream_t st) {
   // an expert has at most T tokens; both kernels need two stages next to a unit's tokens
-  auto fits = [&](int g) { return up_stages(p, g) && down_stages(p, g); };
+  auto fits = [&](int g) {
+    MoeParams q = p;
+    return plan_up(q, g) && plan_down(q, g);
+  };
   if (p.T > 4 && fits(1)) return launch<1>(p, st);
   if (p.T > 2 && fits(2)) return launch<2>(p, st);
   return fits(4) ? launch<4>(p, st) : NPB_ERR_TOO_LARGE;
@@ -1042,9 +1123,6 @@ int make_weight(const npb_q_weight* w, int64_t N, int64_t K, MoeWeight* out) {
   out->group_shift = -1;
   for (int s = 0; s < 16; ++s)
     if (out->group_blocks == 1 << s) out->group_shift = s;
-  // the last group of the last step lies at most eight groups behind the first, which lies at most seven behind
-  // the window's start: sixteen values hold them
-  out->window = out->group_blocks >= 4 ? 8 : 2 * out->group_blocks;
   return NPB_OK;
 }
 
@@ -1062,7 +1140,8 @@ int q_moe_device_status(int* host_out) {
 
 int64_t q_moe_workspace_bytes(int64_t T, int top_k, int64_t I) {
   if (T < 0 || top_k <= 0 || I <= 0 || T > kMaxTokens || top_k > kMaxTopK || I % 32 != 0) return 0;
-  return (int64_t)sizeof(Units) + T * top_k * (I / 32) * kRecord;  // a pair of tokens of an expert is at least one of the T * top_k
+  // a pair of tokens of an expert is at least one of the T * top_k
+  return (int64_t)sizeof(Units) + T * top_k * ((I / 32 + 3) / 4 * 4) * kRecord;
 }
 
 int q_moe(const void* x, int dtype, const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t H, int64_t I,
