@@ -625,7 +625,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
         const int start = window_start<MODE>(p.gate, s0 * 4);
         uint8_t* codes = dyn + stage * kUpCodes;
         const int windows = at.windows + stage * at.window_stage, part = kUpRows * p.window;
-        if (thread == 0) {
+        if (warp == kConsumers && sm100::elect_one()) {
           sm100::mbar_arrive_expect_tx(&full[stage], n * 2 * kUpRows * 64 + (MODE == kAny ? 0 : at.window_stage));
           for (int i = 0; i < n; ++i)
 #pragma unroll
@@ -855,7 +855,7 @@ moe_down_kernel(const __grid_constant__ DownMaps maps, const MoeParams p) {
       const int start = window_start<MODE>(p.down, s0 * 4), pairs = (__popc(lists.mask[u]) + 1) / 2;
       const int windows = at.windows + stage * at.window_stage, part = rows * p.window;
       const uint32_t h_bytes = n * 4 * kRecord;
-      if (thread == 0) {
+      if (warp == kConsumers && sm100::elect_one()) {
         sm100::mbar_arrive_expect_tx(&full[stage], n * rows * 64 + pairs * h_bytes + (MODE == kAny ? 0 : at.window_stage));
         for (int i = 0; i < n; ++i)
           sm100::tma_load_2d(dyn + stage * 512 * 64 + i * rows * 64, &maps.codes, &full[stage], (s0 + i) * 64, row);

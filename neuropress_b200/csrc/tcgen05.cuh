@@ -66,6 +66,19 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// True for one lane of a converged warp.  The compiler knows that it is one: operands of TMA and tcgen05 instructions
+// behind it go to uniform registers directly, where a test of the lane number costs a loop over the lanes each
+// (an issuing thread spent 400 cycles on four MMAs and 500 on two loads).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 // Generic-proxy writes to shared memory -> visible to the async proxy (TMA / tcgen05).
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
