@@ -48,7 +48,8 @@ struct SkinnyParams {
   int rows;       // of x per tile: multiple of 16, at most 256
   int boxes;      // of 64 of k per stage: 1 or 2
   int stages, k_stages, split;
-  int part_rows;  // rows of x whose partial sums fit the ring
+  int part_rows;  // rows of x whose partial sums fit: in the ring, or
+  int part_at;    // behind it, so many bytes from its start (0: in it)
   uint64_t wait_ns;
 };
 
@@ -108,16 +109,20 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   }
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (p.split > 1 && p.part_at != 0) {
+    __syncwarp();
+    cluster_arrive();
+  }
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 1;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&empty[s], ph, abort_flag, p.wait_ns)) {
-          atomicExch(&g_skinny_status, 1);
-          break;
-        }
+    int s = 0;
+    uint32_t ph = 1;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ph, abort_flag, p.wait_ns))) {
+        atomicExch(&g_skinny_status, 1);
+        break;
+      }
+      if (elect_one()) {
         uint8_t* st = ring + (size_t)s * stage_bytes;
         // all bytes of a pair's stage are credited to its even CTA's barrier
         if (side == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * stage_bytes));
@@ -132,38 +137,42 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             tma_load_2d(st + p.boxes * kWBox + h * x_box, &map_x, &full[s], k, m0);
           }
         }
-        if (++s == p.stages) { s = 0; ph ^= 1; }
       }
+      __syncwarp();
+      if (++s == p.stages) { s = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
-    if (lane == 0 && side == 0) {
+    if (side == 0) {
       const uint32_t idesc = umma_idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, CG * BN, p.rows);
       const uint32_t both = 3u << (cta & ~1);
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&full[s], ph, abort_flag, p.wait_ns)) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], ph, abort_flag, p.wait_ns))) {
           atomicExch(&g_skinny_status, 2);
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t st = smem_u32(ring + (size_t)s * stage_bytes);
-        for (int h = 0; h < p.boxes; ++h) {
-          const uint64_t a = umma_desc_sw128(st + h * kWBox), b = umma_desc_sw128(st + p.boxes * kWBox + h * x_box);
+        if (elect_one()) {
+          const uint32_t st = smem_u32(ring + (size_t)s * stage_bytes);
+          for (int h = 0; h < p.boxes; ++h) {
+            const uint64_t a = umma_desc_sw128(st + h * kWBox), b = umma_desc_sw128(st + p.boxes * kWBox + h * x_box);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t more = (kb > kb0 || h > 0 || k > 0) ? 1u : 0u;
-            if (PAIR) umma_f16_pair(tmem, a + 2 * k, b + 2 * k, idesc, more);
-            else umma_f16(tmem, a + 2 * k, b + 2 * k, idesc, more);
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t more = (kb > kb0 || h > 0 || k > 0) ? 1u : 0u;
+              if (PAIR) umma_f16_pair(tmem, a + 2 * k, b + 2 * k, idesc, more);
+              else umma_f16(tmem, a + 2 * k, b + 2 * k, idesc, more);
+            }
           }
+          if (PAIR) umma_commit_pair(&empty[s], both);
+          else umma_commit(&empty[s]);
         }
-        if (PAIR) umma_commit_pair(&empty[s], both);
-        else umma_commit(&empty[s]);
+        __syncwarp();
         if (++s == p.stages) { s = 0; ph ^= 1; }
       }
-      if (ok) {
+      if (ok && elect_one()) {
         if (PAIR) umma_commit_pair(done, both);
         else umma_commit(done);
       }
@@ -203,86 +212,89 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     tc_fence_before();
   } else {
-    // The partial sums go to the ring (every stage has been read), as many rows of x as it holds; each CTA of the
-    // cluster finishes an equal share of them, four outputs of a row at a time, adding them in rank order.
+    // A CTA of the cluster finishes its share of the tile's outputs.  The others push their partial sums of them into
+    // its shared memory, [rank][row of x][share], as many rows of x at a time as fit; it adds them in rank order, four
+    // outputs of a row at a time.
+    struct alignas(8) Four { T e[4]; };
+    constexpr int kAhead = 8;  // units whose residual is on its way
+    const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 &&
+                      (reinterpret_cast<uintptr_t>(p.residual) & 7) == 0;
+    const int share = BN / p.split, units = share / 4, row_step = kThreads / units;
+    const int n = n0 + rank * share + tid % units * 4;  // this thread's outputs
+    float bias[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bias[k] = p.bias && n + k < p.N ? __ldg(p.bias + n + k) : 0.f;
+    Four ahead[kAhead];
+    auto load_residual = [&](int row, int end) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t at = (int64_t)(m0 + row + j * row_step) * p.N + n;
+        const bool in = p.residual != nullptr && row + j * row_step < end;
+        const T* from = static_cast<const T*>(p.residual) + at;
+        if (wide) {
+          if (in && n < p.N) ahead[j] = *reinterpret_cast<const Four*>(from);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (in && n + k < p.N) ahead[j].e[k] = from[k];
+        }
+      }
+    };
+    load_residual(tid / units, min(rows, p.part_rows));
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(done, 0, abort_flag, p.wait_ns, 64u));
     if (!got) atomicExch(&g_skinny_status, 3);
     tc_fence_after();
-    struct alignas(8) Four { T e[4]; };
-    const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 &&
-                      (reinterpret_cast<uintptr_t>(p.residual) & 7) == 0;
-    const uint32_t part = smem_u32(ring);
+    const uint32_t part = smem_u32(ring) + p.part_at;
+    const uint32_t to = map_to_cta(part + (rank * p.part_rows * share + lane_n % share) * 4, lane_n / share * CG + side);
     for (int first = 0; first < rows; first += p.part_rows) {
-      const int here = min(p.part_rows, rows - first), total = here * (BN / 4);
-      if (first > 0) {
-        __syncwarp();
-        cluster_sync_all();  // the rows before are finished
-      }
+      const int here = min(p.part_rows, rows - first);
+      __syncwarp();
+      if (first == 0 && p.part_at != 0) cluster_wait();  // the others have started
+      else cluster_sync_all();  // the others are through with their rings, or with the rows before
       if (got) {
-        float* to = reinterpret_cast<float*>(ring);
         for (int c = c0; c < here; c += 32) {
           uint32_t v[16];
           tmem_ld_32x32_x16(acc + first + c, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) to[(c + i) * BN + lane_n] = __uint_as_float(v[i]);
+          for (int i = 0; i < 16; ++i)
+            if (c + i < here)
+              asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (c + i) * share * 4), "r"(v[i]) : "memory");
         }
       }
-      const int last = (int)((int64_t)total * (rank + 1) / p.split);
-      int i = (int)((int64_t)total * rank / p.split) + tid;
-      float r[4], bias[4];
-      auto load_rest = [&](int u) {
-        const int n = n0 + u % (BN / 4) * 4, m = m0 + first + u / (BN / 4);
+      __syncwarp();
+      cluster_sync_all();
+      for (int row = tid / units; row < here; row += kAhead * row_step) {
+        if (row >= kAhead * row_step || first > 0) load_residual(first + row, first + here);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          bias[k] = p.bias && u < last && n + k < p.N ? __ldg(p.bias + n + k) : 0.f;
-          r[k] = 0.f;
-        }
-        if (p.residual && u < last) {
+        for (int j = 0; j < kAhead; ++j) {
+          const int m = row + j * row_step;
+          if (m >= here) break;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4* from = reinterpret_cast<const float4*>(ring + p.part_at) + m * units + tid % units;
+          for (int c = 0; c < p.split; ++c) {
+            const float4 q = from[c * p.part_rows * units];
+            v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+          }
+          T* y = static_cast<T*>(p.y) + (int64_t)(m0 + first + m) * p.N + n;
+          Four f;
+          const float sum[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float r = p.residual && n + k < p.N ? to_f32(ahead[j].e[k]) : 0.f;
+            f.e[k] = from_f32<T>(activate(sum[k] + bias[k], p.act) + r);
+          }
           if (wide && n < p.N) {
-            const Four f = *reinterpret_cast<const Four*>(static_cast<const T*>(p.residual) + (int64_t)m * p.N + n);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) r[k] = to_f32(f.e[k]);
+            *reinterpret_cast<Four*>(y) = f;
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (n + k < p.N) r[k] = residual_at<T>(p, m, n + k);
+              if (n + k < p.N) y[k] = f.e[k];
           }
         }
-      };
-      load_rest(i);
-      __syncwarp();
-      cluster_sync_all();
-      for (; i < last; i += kThreads) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int c = 0; c < p.split; ++c) {
-          float4 q;
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w)
-                       : "r"(map_to_cta(part + i * 16, c * CG + side))
-                       : "memory");
-          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-        }
-        const int n = n0 + i % (BN / 4) * 4, m = m0 + first + i / (BN / 4);
-        T* y = static_cast<T*>(p.y) + (int64_t)m * p.N + n;
-        Four f;
-        const float sum[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f.e[k] = from_f32<T>(activate(sum[k] + bias[k], p.act) + r[k]);
-        if (wide && n < p.N) {
-          *reinterpret_cast<Four*>(y) = f;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n + k < p.N) y[k] = f.e[k];
-        }
-        load_rest(i + kThreads);
       }
     }
     tc_fence_before();
-    __syncwarp();
-    cluster_sync_all();  // nobody leaves while its sums are read
   }
   if (*abort_flag) {
     const uint64_t t0 = global_timer_ns();
@@ -391,8 +403,10 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
     if (tiles * row_tiles * p.split * 2 > most) break;
     p.split *= 2;
   }
-  const int ring = p.stages * stage_bytes;
-  p.part_rows = ring / (BN * 4) / 32 * 32;
+  const int ring = p.stages * stage_bytes, most_rows = (int)(M < p.rows ? M : p.rows);
+  const bool behind = p.split > 1 && ring + most_rows * BN * 4 <= room;  // partial sums that need no wait for the ring
+  p.part_at = behind ? ring : 0;
+  p.part_rows = behind ? most_rows : ring / (BN * 4) / 32 * 32;
   const bool bf16 = dtype == NPB_BF16;
   CUtensorMap map_w, map_x;
   const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -401,7 +415,7 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)row_tiles);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 1024 + kHead + ring;
+  cfg.dynamicSmemBytes = 1024 + kHead + ring + (behind ? most_rows * BN * 4 : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
