@@ -24,4 +24,20 @@ __device__ __forceinline__ float activate(float v, int act) {
   }
 }
 
+// One branch for all of them: the values' chains overlap.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], int act) {
+  auto each = [&](int which) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = activate(v[i], which);
+  };
+  switch (act) {
+    case NPB_ACT_RELU: return each(NPB_ACT_RELU);
+    case NPB_ACT_SILU: return each(NPB_ACT_SILU);
+    case NPB_ACT_GELU: return each(NPB_ACT_GELU);
+    case NPB_ACT_GELU_TANH: return each(NPB_ACT_GELU_TANH);
+    default: return;
+  }
+}
+
 }  // namespace npb

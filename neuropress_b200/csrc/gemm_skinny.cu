@@ -201,7 +201,10 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         T* y = static_cast<T*>(p.y) + (int64_t)(m0 + c) * p.N + n0 + lane_n;
         float o[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = activate(__uint_as_float(v[i]) + bias, p.act) + r[i];
+        for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(v[i]) + bias;
+        activate_all(o, p.act);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] += r[i];
         load_residual(c + 32);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -216,7 +219,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     // its shared memory, [rank][row of x][share], as many rows of x at a time as fit; it adds them in rank order, four
     // outputs of a row at a time.
     struct alignas(8) Four { T e[4]; };
-    constexpr int kAhead = 8;  // units whose residual is on its way
+    constexpr int kAhead = 16;  // units of a thread, at most (256 rows, a split in two)
     const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 &&
                       (reinterpret_cast<uintptr_t>(p.residual) & 7) == 0;
     const int share = BN / p.split, units = share / 4, row_step = kThreads / units;
@@ -224,33 +227,45 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     float bias[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) bias[k] = p.bias && n + k < p.N ? __ldg(p.bias + n + k) : 0.f;
-    Four ahead[kAhead];
-    auto load_residual = [&](int row, int end) {
+    Four rest[kAhead];  // the residual: fetched before the sums are there, kept in shared memory while they are joined
+    auto fetch = [&](int j) {
+      rest[j] = Four{};
+      const int row = tid / units + j * row_step;
+      if (p.residual == nullptr || row >= rows) return;
+      const T* from = static_cast<const T*>(p.residual) + (int64_t)(m0 + row) * p.N + n;
+      if (wide) {
+        if (n < p.N) rest[j] = *reinterpret_cast<const Four*>(from);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int64_t at = (int64_t)(m0 + row + j * row_step) * p.N + n;
-        const bool in = p.residual != nullptr && row + j * row_step < end;
-        const T* from = static_cast<const T*>(p.residual) + at;
-        if (wide) {
-          if (in && n < p.N) ahead[j] = *reinterpret_cast<const Four*>(from);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (in && n + k < p.N) ahead[j].e[k] = from[k];
-        }
+        for (int k = 0; k < 4; ++k)
+          if (n + k < p.N) rest[j].e[k] = from[k];
       }
     };
-    load_residual(tid / units, min(rows, p.part_rows));
+    const bool more = rows > row_step;  // few rows skip the code for many
+    fetch(0);
+    if (more) {
+#pragma unroll
+      for (int j = 1; j < kAhead; ++j) fetch(j);
+    }
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(done, 0, abort_flag, p.wait_ns, 64u));
     if (!got) atomicExch(&g_skinny_status, 3);
     tc_fence_after();
     const uint32_t part = smem_u32(ring) + p.part_at;
+    Four* kept = reinterpret_cast<Four*>(ring + p.part_at + p.part_rows * BN * 4);  // [row][units]
     const uint32_t to = map_to_cta(part + (rank * p.part_rows * share + lane_n % share) * 4, lane_n / share * CG + side);
     for (int first = 0; first < rows; first += p.part_rows) {
       const int here = min(p.part_rows, rows - first);
       __syncwarp();
       if (first == 0 && p.part_at != 0) cluster_wait();  // the others have started
       else cluster_sync_all();  // the others are through with their rings, or with the rows before
+      if (first == 0) {
+        if (tid / units < rows) kept[tid] = rest[0];
+        if (more) {
+#pragma unroll
+          for (int j = 1; j < kAhead; ++j)
+            if (tid / units + j * row_step < rows) kept[j * kThreads + tid] = rest[j];
+        }
+      }
       if (got) {
         for (int c = c0; c < here; c += 32) {
           uint32_t v[16];
@@ -264,33 +279,40 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
       __syncwarp();
       cluster_sync_all();
-      for (int row = tid / units; row < here; row += kAhead * row_step) {
-        if (row >= kAhead * row_step || first > 0) load_residual(first + row, first + here);
+      const float4* from = reinterpret_cast<const float4*>(ring + p.part_at) + tid;
+#pragma unroll 1  // a short body: it runs a few times, and fetching it costs more than running it
+      for (int row = tid / units; row < here; row += 2 * row_step, from += 2 * kThreads) {
+        const bool two = row + row_step < here;
+        const int next = two ? kThreads : 0;
+        float sum[8];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const int m = row + j * row_step;
-          if (m >= here) break;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          const float4* from = reinterpret_cast<const float4*>(ring + p.part_at) + m * units + tid % units;
-          for (int c = 0; c < p.split; ++c) {
-            const float4 q = from[c * p.part_rows * units];
-            v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-          }
-          T* y = static_cast<T*>(p.y) + (int64_t)(m0 + first + m) * p.N + n;
+        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+#pragma unroll 2
+        for (int c = 0; c < p.split; ++c) {
+          const float4 q = from[c * p.part_rows * units], r = from[c * p.part_rows * units + next];
+          sum[0] += q.x; sum[1] += q.y; sum[2] += q.z; sum[3] += q.w;
+          sum[4] += r.x; sum[5] += r.y; sum[6] += r.z; sum[7] += r.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += bias[k & 3];
+        activate_all(sum, p.act);
+        const Four* rest = kept + (first + row) * units + tid % units;
+        T* y = static_cast<T*>(p.y) + (int64_t)(m0 + first + row) * p.N + n;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const Four r = rest[j * next];
           Four f;
-          const float sum[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float r = p.residual && n + k < p.N ? to_f32(ahead[j].e[k]) : 0.f;
-            f.e[k] = from_f32<T>(activate(sum[k] + bias[k], p.act) + r);
-          }
-          if (wide && n < p.N) {
-            *reinterpret_cast<Four*>(y) = f;
+          for (int k = 0; k < 4; ++k) f.e[k] = from_f32<T>(sum[j * 4 + k] + to_f32(r.e[k]));
+          if (j == 1 && !two) break;
+          if (wide) {
+            if (n < p.N) *reinterpret_cast<Four*>(y) = f;
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               if (n + k < p.N) y[k] = f.e[k];
           }
+          y += (int64_t)row_step * p.N;
         }
       }
     }
@@ -404,9 +426,10 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
     p.split *= 2;
   }
   const int ring = p.stages * stage_bytes, most_rows = (int)(M < p.rows ? M : p.rows);
-  const bool behind = p.split > 1 && ring + most_rows * BN * 4 <= room;  // partial sums that need no wait for the ring
+  const int rest = most_rows * (BN / p.split) * 2;  // the residual's share
+  const bool behind = p.split > 1 && ring + most_rows * BN * 4 + rest <= room;  // partial sums need no wait for the ring
   p.part_at = behind ? ring : 0;
-  p.part_rows = behind ? most_rows : ring / (BN * 4) / 32 * 32;
+  p.part_rows = behind ? most_rows : (ring - rest) / (BN * 4) / 32 * 32;
   const bool bf16 = dtype == NPB_BF16;
   CUtensorMap map_w, map_x;
   const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -415,7 +438,7 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)row_tiles);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 1024 + kHead + ring + (behind ? most_rows * BN * 4 : 0);
+  cfg.dynamicSmemBytes = 1024 + kHead + ring + (behind ? most_rows * BN * 4 + rest : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;

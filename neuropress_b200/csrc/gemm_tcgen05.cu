@@ -424,13 +424,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
               }
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
+                float f[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                  float f = __uint_as_float(v[q * 8 + e]);
-                  if (p.bias) f += __ldg(p.bias + n0 + q * 8 + e);
-                  if (EPI) f = activate(f, p.act);
-                  if (EPI && res) f += to_f32(o[q].e[e]);
-                  o[q].e[e] = from_f32<T>(f);
+                  f[e] = __uint_as_float(v[q * 8 + e]);
+                  if (p.bias) f[e] += __ldg(p.bias + n0 + q * 8 + e);
+                }
+                if (EPI) activate_all(f, p.act);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  if (EPI && res) f[e] += to_f32(o[q].e[e]);
+                  o[q].e[e] = from_f32<T>(f[e]);
                 }
               }
               Out* dst = reinterpret_cast<Out*>(y + off);
