@@ -380,13 +380,18 @@ int resident_ctas(int cluster, int* ctas) {
   return NPB_OK;
 }
 
-// Whether this form is the faster one: up to 256 rows for every N, and above where the dense kernel's tiles leave SMs
-// idle -- up to 64 tiles in all (512 x 2048 x 8192: 29 / 50 us; 1024 x 8192 x 8192 with 256: 182 / 126 us), or one wave
-// of them with fewer rows each (400 x 8192 x 8192: 87 / 92 us; 512: 95 / 84 us).
-bool gemm_skinny_takes(int64_t M, int64_t N) {
+// Whether this form is the faster one (this / the dense kernel, us): while tiles can be split over the SMs (256 rows, 4096 x
+// 14336: 38 / 78; 512 rows, 2048 x 8192: 24 / 50); in one wave of tiles if they are not too high (128 rows, 14336 x 4096:
+// 32 / 34; 256 rows: 43 / 41); in two waves, which the dense kernel's epilogue overlaps, with few rows (64 rows, 32000 x
+// 4096: 53 / 55; 96 rows: 58 / 55) or long sums (201 rows, 28672 x 8192: 116 / 153; 96 rows, 36864 x 8192: 108 / 109); and
+// with a few rows always (16 rows, 49152 x 4096: 72 / 76; 48 rows: 88 / 77).
+bool gemm_skinny_takes(int64_t M, int64_t N, int64_t K) {
   const int64_t row_tiles = (M + 255) / 256, all = row_tiles * ((N + BN - 1) / BN);
   const int64_t rows = row_tiles ? (M + row_tiles - 1) / row_tiles : 0;
-  return row_tiles <= 1 || all <= 64 || (all <= sm_count() && rows <= 208);
+  if (all * 2 <= sm_count()) return true;
+  if (all <= sm_count()) return rows <= 208;
+  if (row_tiles > 1) return false;
+  return rows <= (all > 2 * sm_count() ? 32 : K < 8192 ? 64 : 208);
 }
 
 // Tiles of at most 256 rows of x; W is read once per tile of rows.
@@ -399,17 +404,19 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   p.M = (int)M; p.N = (int)N; p.act = act;
   const int row_tiles = (int)((M + 255) / 256);
   const int rows = (int)((M + row_tiles - 1) / row_tiles);
-  // Pairs where more than 128 rows meet so many tiles that a split in two will do (201 rows, 14336 x 4096: 49 us against
-  // 59 us without; 128 rows: 38 / 36 us).  Split further they need clusters of eight, two CTAs to an SM, on half of the
-  // SMs (201 rows, 4096 x 14336: 53 / 40 us).
-  const bool pair = rows > 128 && (N + BN - 1) / BN >= 96;
+  const int64_t tiles_1 = (N + BN - 1) / BN * row_tiles;  // of one CTA
+  const int half = max_dynamic_smem() / 2 - 1024 - 2048, whole = max_dynamic_smem() - 2048;
+  auto two_fit = [&](int x_rows) { return (half - kHead) / (kWBox + x_rows * 128) >= 3; };  // CTAs on an SM
+  // Too many tiles for a split in two, one CTA to an SM: two CTAs to an SM (128 rows, 14336 x 4096: 32 us, one to an SM
+  // 39 us), or pairs where the rows leave room for one (201 rows, 14336 x 4096: 39 us against 52 us without; 400 rows, 8192 x
+  // 8192: 57 / 69 us).  Otherwise one CTA with the whole ring is better (128 rows, 4096 x 4096: 14.8 us, two to an SM
+  // 16.3 us), and pairs cost: they need clusters of eight, on fewer SMs (201 rows, 4096 x 14336: 63 / 34 us).
+  const bool crowded = tiles_1 * 2 > sm_count(), pair = crowded && !two_fit((rows + 15) / 16 * 16);
   const int cg = pair ? 2 : 1, step = 16 * cg;
   p.rows = (rows + step - 1) / step * step;
   p.wait_ns = wait_limit_ns();
   const int box_bytes = kWBox + p.rows / cg * 128;  // of W and x, 64 of k
-  // two CTAs on an SM where three boxes of each fit
-  const int half = max_dynamic_smem() / 2 - 1024 - 2048, whole = max_dynamic_smem() - 2048;
-  const int per_sm = (half - kHead) / box_bytes >= 3 ? 2 : 1, room = (per_sm == 2 ? half : whole) - kHead;
+  const int per_sm = crowded && two_fit(p.rows / cg) ? 2 : 1, room = (per_sm == 2 ? half : whole) - kHead;
   p.boxes = room / box_bytes >= 6 ? 2 : 1;
   const int stage_bytes = p.boxes * box_bytes;
   p.stages = room / stage_bytes < kMaxStages ? room / stage_bytes : kMaxStages;
@@ -419,8 +426,7 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   while (p.split * cg < (pair ? 4 : 8) && p.k_stages >= p.split * 4) {
     int room_for = 0;  // CTAs that run at once, one to an SM, in clusters of twice the size
     if (int rc = resident_ctas(p.split * cg * 2, &room_for)) return rc;
-    // a tenth more than run at once is better than half as many where two share an SM (1 row, 4096 x 14336: 256 CTAs
-    // 24 us, 128 CTAs 25 us), and worse where they do not (256 rows, 2048 x 2048: 128 CTAs 24 us, 64 CTAs 19 us)
+    // where two share an SM a tenth more than run at once is better than half as many
     const int64_t most = per_sm == 2 ? room_for * 2 * 11 / 10 : room_for;
     if (tiles * row_tiles * p.split * 2 > most) break;
     p.split *= 2;

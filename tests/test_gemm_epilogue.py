@@ -75,6 +75,23 @@ def test_shapes(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [
+    (1, 9601, 264), (3, 19200, 136), (33, 9480, 4104), (100, 9601, 520), (128, 18944, 264), (150, 12801, 2056),
+    (161, 9475, 1032), (176, 9600, 8192), (201, 12803, 4104), (208, 18432, 136), (256, 9481, 264), (256, 9216, 1096),
+    (300, 8192, 520), (400, 8190, 2056), (416, 9344, 72), (30, 40000, 264), (33, 40001, 264), (201, 20000, 8200)])
+def test_many_tiles(shape):
+    """CTA pairs, two CTAs to an SM and the sizes where the forms change over, with odd and even rows of outputs."""
+    m, n, k = shape
+    x, w, b, r = make(m, n, k, torch.bfloat16, seed=m + n + k)
+    y = run(x, w, b, "gelu", r)
+    assert_output_close(y, plain(x, w, b, "gelu", r, DEV), torch.bfloat16, tol=TOL)
+    assert torch.equal(y, run(x, w, b, "gelu", r))
+    x, w, b, r = make(m, n, k, torch.float16, seed=m + n + k, bias=False)
+    assert_output_close(run(x, w, b, "none", r), plain(x, w, b, "none", r, DEV), torch.float16, tol=TOL)
+    assert _cabi.gemm_device_status() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 40, 140, 400])
 def test_plain_product_agrees_with_gemm(m):
     x, w, b, _ = make(m, 1024, 2048, torch.bfloat16, seed=m)
