@@ -5,7 +5,7 @@
 //   the n largest l_v, equal values by ascending v, as log p_v and v
 //
 // A row is split over a cluster of 1..8 CTAs; each thread keeps (m, s, u) of its own elements with a
-// running maximum (a tile of three 16-byte loads raises m at most once), so every logit is read from
+// running maximum (a tile of three or eight 16-byte loads raises m at most once), so every logit is read from
 // HBM once.  All sums are fp32; l - m is formed before the multiplication by log2(e), so rows with a
 // large common offset lose nothing.  Bound by HBM for many rows, by latency for a few.
 //
@@ -20,6 +20,8 @@
 // Per element of a 16-bit row: one unpacking, half an instruction each for the maximum (on packed pairs), l - m, its
 // scaling, and the two sums (packed fp32), one ex2.  The exponentials alone would take 0.7 of the time that HBM
 // needs for them.
+#include <type_traits>
+
 #include "common.cuh"
 #include "order_key.cuh"
 #include "tcgen05.cuh"
@@ -34,7 +36,8 @@ using sm100::smem_u32;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 3;      // 16-byte loads per thread and tile
+constexpr int kUnroll = 3;      // 16-byte loads per thread and tile with many rows
+constexpr int kWide = 8;        // and with few
 constexpr int kMaxTop = 32;
 constexpr int kListCap = 1024;  // candidate keys in shared memory
 constexpr int kMaxSplit = 8;    // CTAs per row (portable cluster size)
@@ -71,6 +74,7 @@ __device__ __forceinline__ Part merge(const Part& a, const Part& b) {
 template <typename T>
 struct Tile {
   static constexpr int EPV = 16 / (int)sizeof(T);
+  static constexpr uint32_t kMasked = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
   struct alignas(16) Vec { T e[EPV]; };
 };
 
@@ -127,9 +131,9 @@ __device__ __forceinline__ float largest(const Tile<__nv_bfloat16>::Vec& q) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
-// Adds N vectors to a part.  The product e * d is 0 * -inf = NaN for a masked (-inf) element; such a tile (u is NaN,
+// Adds N vectors to a part.  CLAMP: any of them may be masked.  Otherwise the product e * d is 0 * -inf = NaN for a masked (-inf) element; such a tile (u is NaN,
 // s is not) is summed again with d clamped, so that the others pay nothing.
-template <typename T, int N>
+template <typename T, int N, bool CLAMP>
 __device__ __forceinline__ void add_vectors(Part& p, const typename Tile<T>::Vec (&q)[N]) {
   constexpr int PAIRS = Tile<T>::EPV / 2;
   float tm = largest(q[0]);
@@ -148,11 +152,15 @@ __device__ __forceinline__ void add_vectors(Part& p, const typename Tile<T>::Vec
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int k = 0; k < PAIRS; ++k) {
-      const F2 d = add2(pair_of<T>(q[i], k), less);
+      F2 d = add2(pair_of<T>(q[i], k), less);
       float a, b;
       unpack(mul2(d, scale), a, b);
       const F2 e = pack(ex2(a), ex2(b));
       s2 = add2(s2, e);
+      if (CLAMP) {
+        unpack(d, a, b);
+        d = pack(fmaxf(a, -1e20f), fmaxf(b, -1e20f));
+      }
       u2 = fma2(e, d, u2);
     }
   float s, s_hi, u, u_hi;
@@ -160,7 +168,7 @@ __device__ __forceinline__ void add_vectors(Part& p, const typename Tile<T>::Vec
   unpack(u2, u, u_hi);
   s += s_hi;
   u += u_hi;
-  if (u != u) {
+  if (!CLAMP && u != u) {
     u = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -263,10 +271,10 @@ __device__ void select_by_bisection(const T* __restrict__ row, int first, int la
   __syncthreads();
 }
 
-// Six CTAs on an SM: what hides the loads is occupancy (4096 x 128000 bf16: 187 us, 5.6 TB/s; four CTAs with four loads
+// Six CTAs on an SM with many rows: what hides the loads is occupancy (4096 x 128000 bf16: 187 us, 5.6 TB/s; four CTAs with four loads
 // per tile 194 us, three with the next tile prefetched into registers 249 us).
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 6)
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kThreads, WIDE ? 3 : 6)
 token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ targets, int top_n,
                       int split, float* __restrict__ logprob, float* __restrict__ entropy,
                       float* __restrict__ top_logprobs, int64_t* __restrict__ top_ids) {
@@ -291,15 +299,32 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
   Part p{-INFINITY, 0.f, 0.f};
   const T* vectors = row + head;
   int v = v0 + tid;
-  for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
-    typename Tile<T>::Vec q[kUnroll];
+  if (WIDE) {
+    for (; v < v1; v += kWide * kThreads) {
+      typename Tile<T>::Vec q[kWide];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) q[i] = load_vec(vectors + (int64_t)(v + i * kThreads) * EPV);
-    add_vectors<T>(p, q);
-  }
-  for (; v < v1; v += kThreads) {
-    const typename Tile<T>::Vec q[1] = {load_vec(vectors + (int64_t)v * EPV)};
-    add_vectors<T>(p, q);
+      for (int i = 0; i < kWide; ++i) {
+        if (v + i * kThreads < v1) {
+          q[i] = load_vec(vectors + (int64_t)(v + i * kThreads) * EPV);
+        } else {  // masked elements
+          const uint32_t f = Tile<T>::kMasked;
+          const uint4 none = make_uint4(f, f, f, f);
+          q[i] = *reinterpret_cast<const typename Tile<T>::Vec*>(&none);
+        }
+      }
+      add_vectors<T, kWide, true>(p, q);
+    }
+  } else {
+    for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
+      typename Tile<T>::Vec q[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) q[i] = load_vec(vectors + (int64_t)(v + i * kThreads) * EPV);
+      add_vectors<T, kUnroll, false>(p, q);
+    }
+    for (; v < v1; v += kThreads) {
+      const typename Tile<T>::Vec q[1] = {load_vec(vectors + (int64_t)v * EPV)};
+      add_vectors<T, 1, false>(p, q);
+    }
   }
   if (odd >= 0) p = merge(p, part_of(to_f32(row[odd])));
 
@@ -455,10 +480,15 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
   }
 }
 
-// CTAs per row: as many as keep the GPU busy with few rows, each with a slice worth its start.
+// The wide form holds three CTAs on an SM; a grid of one wave of it has one load latency per eight loads of a thread and
+// none for a ragged end (20 x 128000 bf16: 10.0 us, narrow 10.8 us; 220 x 128000: 23 / 29 us; 150 x 50001 fp32: 15.7 / 16.3
+// us).  More rows have enough CTAs to hide the loads.
+constexpr int kWidePerSm = 3;
+
+// CTAs per row: as many as one wave of the wide form has, each with a slice worth its start.
 int pick_split(int64_t R, int64_t V) {
   int split = 1;
-  while (split < kMaxSplit && R * split * 2 <= (int64_t)sm_count() * 6 && V / (split * 2) >= 2048) split *= 2;
+  while (split < kMaxSplit && R * split * 2 <= (int64_t)sm_count() * kWidePerSm && V / (split * 2) >= 2048) split *= 2;
   return split;
 }
 
@@ -478,8 +508,10 @@ int launch(const void* logits, int64_t ld, int64_t R, int64_t V, const int64_t* 
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, static_cast<const T*>(logits), ld, (int)V, targets,
-                                  top_n, split, logprob, entropy, top_logprobs, top_ids));
+  const bool wide = R * split <= (int64_t)sm_count() * kWidePerSm;
+  NPB_CUDA_TRY(cudaLaunchKernelEx(&cfg, wide ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>,
+                                  static_cast<const T*>(logits), ld, (int)V, targets, top_n, split, logprob, entropy,
+                                  top_logprobs, top_ids));
   NPB_LAUNCH_CHECK();
   return NPB_OK;
 }

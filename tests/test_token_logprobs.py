@@ -115,6 +115,37 @@ def test_masked_and_degenerate_rows(v, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [3001, 6150])
+def test_masked_rows_among_many(v, dtype):
+    """The form for many rows, whose sums treat masked elements apart."""
+    logits, targets = make(10, v, dtype, seed=v)
+    lowest = torch.finfo(dtype).min
+    logits[0] = -math.inf
+    logits[1, ::2] = -math.inf
+    logits[2, 5:] = -math.inf
+    logits[3, : v - 2] = -math.inf
+    logits[4, 1::3] = lowest
+    logits[5, v // 2] = math.nan
+    logits[6, v // 3] = math.inf
+    logits[7, v // 2:] = -math.inf
+    logits[8, : v // 2] = lowest
+    targets[2] = v - 1
+    many, t = logits.repeat(60, 1), targets.repeat(60)
+    check(many[290:310], t[290:310], 20)             # few rows
+    whole = kernels.token_logprobs(many, t, top_n=20)
+    few = kernels.token_logprobs(logits, targets, top_n=20)
+    ref = plain(logits, targets, 20)
+    for w, f in zip(whole, few):
+        # a row is split by how its start is aligned, the same way for every eighth copy of ten rows of 2 or 4 bytes
+        # an element (80 V elements are whole vectors): those have the same bits
+        w = w.view(60, *f.shape).nan_to_num(7.0)
+        assert torch.equal(w[8:], w[:52])
+    check(many, t, 20)
+    assert torch.equal(whole[3][:10].cpu(), ref[3]) and torch.equal(few[3].cpu(), ref[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_large_values_on_one_thread_and_large_offsets(dtype):
     """Large values that all fall to one thread's share, and a common offset far from zero."""
     logits, targets = make(3, 65536 * 2, dtype, seed=4)
