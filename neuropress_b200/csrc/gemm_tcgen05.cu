@@ -260,8 +260,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
-    // ================= TMA producer =================
-    if (lane == 0) {
+    // ================= TMA producer (an elected lane of a converged warp) =================
+    {
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -271,35 +271,38 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         int tm, tn;
         tile_coords(p, t, tm, tn);
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait_bounded(&empty_bar[s], ph ^ 1, abort_flag, p.wait_ns,
-                                 BMODE == B_TMA ? 0u : 128u)) {
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty_bar[s], ph ^ 1, abort_flag, p.wait_ns,
+                                                         BMODE == B_TMA ? 0u : 128u))) {
             atomicExch(&g_gemm_status, 1);
             ok = false;
             break;
           }
-          uint8_t* st = stage_base + (size_t)s * kStageBytes;
-          constexpr uint32_t tx = MT * kAStageBytes + (BMODE == B_TMA ? BN * BK * 2 : 0);
-          if (CG == 2) {
-            if (cta_rank == 0) mbar_arrive_expect_tx(&full_bar[s], tx + kAStageBytes);  // 2 A tiles + all of B
-            const uint32_t bar = full0 + (uint32_t)s * 8u;
-            tma_load_2d_pair(st, &tmap_a, bar, kb * BK, (tm * 2 + cta_rank) * BM);
-            tma_load_2d_pair(st + kAStageBytes, &tmap_b, bar, kb * BK, tn * BN + cta_rank * (BN / 2));
-          } else {
-            mbar_arrive_expect_tx(&full_bar[s], tx);
+          if (elect_one()) {
+            uint8_t* st = stage_base + (size_t)s * kStageBytes;
+            constexpr uint32_t tx = MT * kAStageBytes + (BMODE == B_TMA ? BN * BK * 2 : 0);
+            if (CG == 2) {
+              if (cta_rank == 0) mbar_arrive_expect_tx(&full_bar[s], tx + kAStageBytes);  // 2 A tiles + all of B
+              const uint32_t bar = full0 + (uint32_t)s * 8u;
+              tma_load_2d_pair(st, &tmap_a, bar, kb * BK, (tm * 2 + cta_rank) * BM);
+              tma_load_2d_pair(st + kAStageBytes, &tmap_b, bar, kb * BK, tn * BN + cta_rank * (BN / 2));
+            } else {
+              mbar_arrive_expect_tx(&full_bar[s], tx);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-              tma_load_2d(st + mt * kAStageBytes, &tmap_a, &full_bar[s], kb * BK,
-                          (tm * MT + mt) * BM);
-            if (BMODE == B_TMA)
-              tma_load_2d(st + MT * kAStageBytes, &tmap_b, &full_bar[s], kb * BK, tn * BN);
+              for (int mt = 0; mt < MT; ++mt)
+                tma_load_2d(st + mt * kAStageBytes, &tmap_a, &full_bar[s], kb * BK,
+                            (tm * MT + mt) * BM);
+              if (BMODE == B_TMA)
+                tma_load_2d(st + MT * kAStageBytes, &tmap_b, &full_bar[s], kb * BK, tn * BN);
+            }
           }
+          __syncwarp();
           if (++s == stages) { s = 0; ph ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
     // ================= MMA issuer =================
-    if (lane == 0 && cta_rank == 0) {
+    if (cta_rank == 0) {
       int s = 0;
       uint32_t ph = 0;
       int it = 0;
@@ -307,40 +310,43 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       for (int t = first_tile; t < num_tiles && ok; t += tile_stride, ++it) {
         const int buf = (NBUF == 2) ? (it & 1) : 0;
         const uint32_t buf_ph = (NBUF == 2) ? ((it >> 1) & 1) : (it & 1);
-        if (!mbar_wait_bounded(&tmem_empty[buf], buf_ph ^ 1, abort_flag, p.wait_ns)) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tmem_empty[buf], buf_ph ^ 1, abort_flag, p.wait_ns))) {
           atomicExch(&g_gemm_status, 2);
           break;
         }
         tc_fence_after();
         const uint32_t acc = tmem_base + buf * BUF_STRIDE;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait_bounded(&full_bar[s], ph, abort_flag, p.wait_ns)) {
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[s], ph, abort_flag, p.wait_ns))) {
             atomicExch(&g_gemm_status, 2);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t st = smem_u32(stage_base + (size_t)s * kStageBytes);
-          const uint64_t bdesc = umma_desc_sw128(st + MT * kAStageBytes);
+          if (elect_one()) {
+            const uint32_t st = smem_u32(stage_base + (size_t)s * kStageBytes);
+            const uint64_t bdesc = umma_desc_sw128(st + MT * kAStageBytes);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const uint64_t adesc = umma_desc_sw128(st + mt * kAStageBytes);
+            for (int mt = 0; mt < MT; ++mt) {
+              const uint64_t adesc = umma_desc_sw128(st + mt * kAStageBytes);
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k) {
-              // +32 bytes per K step inside the 128-byte swizzle row: +2 in the >>4 field
-              if (CG == 2)
-                umma_f16_pair(acc, adesc + 2 * k, bdesc + 2 * k, kIdesc, (kb > 0 || k > 0) ? 1u : 0u);
-              else
-                umma_f16(acc + mt * BN, adesc + 2 * k, bdesc + 2 * k, kIdesc,
-                         (kb > 0 || k > 0) ? 1u : 0u);
+              for (int k = 0; k < BK / UMMA_K; ++k) {
+                // +32 bytes per K step inside the 128-byte swizzle row: +2 in the >>4 field
+                if (CG == 2)
+                  umma_f16_pair(acc, adesc + 2 * k, bdesc + 2 * k, kIdesc, (kb > 0 || k > 0) ? 1u : 0u);
+                else
+                  umma_f16(acc + mt * BN, adesc + 2 * k, bdesc + 2 * k, kIdesc,
+                           (kb > 0 || k > 0) ? 1u : 0u);
+              }
             }
+            // frees the stage (in both CTAs of a pair) once these MMAs have read it
+            if (CG == 2) umma_commit_pair(&empty_bar[s]);
+            else umma_commit(&empty_bar[s]);
           }
-          // frees the stage (in both CTAs of a pair) once these MMAs have read it
-          if (CG == 2) umma_commit_pair(&empty_bar[s]);
-          else umma_commit(&empty_bar[s]);
+          __syncwarp();
           if (++s == stages) { s = 0; ph ^= 1; }
         }
-        if (ok) {
+        if (ok && elect_one()) {
           if (CG == 2) umma_commit_pair(&tmem_full[buf]);
           else umma_commit(&tmem_full[buf]);
         }
@@ -359,6 +365,26 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     const int64_t ld = gathered ? p.sink.ld : p.N;
     const int64_t col0 = gathered ? p.sink.col0 : 0;
     if (gathered) y = static_cast<T*>(p.sink.peer_out[p.sink.rank]);
+    struct alignas(16) Out { T e[8]; };
+    constexpr int kChunks = BN / 32, kAhead = EPI && kChunks > 1 ? 2 : 1;  // 32 outputs of a row
+    const T* res = EPI ? static_cast<const T*>(p.residual) : nullptr;
+    // 16-byte accesses only where the address itself is 16-byte aligned (a tensor that is a view at an odd offset takes
+    // the element-wise path)
+    auto whole = [&](int64_t off, int n0) {
+      return n0 + 32 <= p.N && ((reinterpret_cast<uintptr_t>(y + off) & 15u) == 0) &&
+             (!(EPI && res) || (reinterpret_cast<uintptr_t>(res + off) & 15u) == 0);
+    };
+    // The residual of a chunk is on its way while the chunk before the last one is finished, a tile's first two while
+    // the tile is waited for.
+    Out ahead[kAhead][4];
+    auto fetch = [&](int tm, int tn, int mt, int c, Out (&o)[4]) {
+      const int m = (tm * MT + mt) * BM + quad * 32 + lane, n0 = tn * BN + c * 32;
+      const int64_t off = (int64_t)m * ld + col0 + n0;
+      if (res && m < p.M && n0 < p.N && whole(off, n0)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = reinterpret_cast<const Out*>(res + off)[q];
+      }
+    };
     int it = 0;
     bool ok = true;
     const uint32_t empty0 = CG == 2 ? map_to_cta(smem_u32(&tmem_empty[0]), 0) : 0u;  // the leader's
@@ -368,6 +394,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       if (CG == 2) tm = tm * 2 + cta_rank;  // this CTA's 128 rows of the pair's 256
       const int buf = (NBUF == 2) ? (it & 1) : 0;
       const uint32_t buf_ph = (NBUF == 2) ? ((it >> 1) & 1) : (it & 1);
+      if (EPI) {
+        fetch(tm, tn, 0, 0, ahead[0]);
+        if (kChunks > 1) fetch(tm, tn, 0, 1, ahead[kAhead - 1]);
+      }
       // All lanes wait (each needs the acquire), then agree on the outcome so that the
       // warp-collective tcgen05.ld below is never reached by part of a warp.
       const bool got = mbar_wait_bounded(&tmem_full[buf], buf_ph, abort_flag, p.wait_ns,
@@ -400,28 +430,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         // Rows past M hold zeros (TMA zero fill); whole sub-tiles past M are skipped by all
         // lanes together so the tcgen05.ld stays warp-uniform.
         if ((tm * MT + mt) * BM >= p.M) break;
-#pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
+        auto finish = [&](int c, Out (&o)[4]) {
           uint32_t v[32];
           tmem_ld_32x32(acc + mt * BN + c * 32, v);
           tmem_ld_wait();
           const int n0 = tn * BN + c * 32;
           if (m < p.M && n0 < p.N) {
             const int64_t off = (int64_t)m * ld + col0 + n0;
-            // 16-byte stores only where the destination address itself is 16-byte aligned (an
-            // output that is a view at an odd offset takes the element-wise path)
-            bool full = (n0 + 32 <= p.N) && ((reinterpret_cast<uintptr_t>(y + off) & 15u) == 0);
-            const T* res = EPI ? static_cast<const T*>(p.residual) : nullptr;
-            if (EPI && res) {
-              res += off;
-              full = full && (reinterpret_cast<uintptr_t>(res) & 15u) == 0;
-            }
-            if (full) {
-              struct alignas(16) Out { T e[8]; } o[4];
-              if (EPI && res) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) o[q] = reinterpret_cast<const Out*>(res)[q];
-              }
+            if (whole(off, n0)) {
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float f[8];
@@ -448,12 +464,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                   float f = __uint_as_float(v[e]);
                   if (p.bias) f += __ldg(p.bias + n0 + e);
                   if (EPI) f = activate(f, p.act);
-                  if (EPI && res) f += to_f32(res[e]);
+                  if (EPI && res) f += to_f32(res[off + e]);
                   dst[e] = from_f32<T>(f);
                 }
               }
             }
           }
+        };
+#pragma unroll 1
+        for (int c = 0; c < kChunks; c += kAhead) {
+          finish(c, ahead[0]);
+          if (EPI && c + 2 < kChunks) fetch(tm, tn, mt, c + 2, ahead[0]);
+          if (kAhead == 1 || c + 1 == kChunks) continue;
+          finish(c + 1, ahead[kAhead - 1]);
+          if (EPI && c + 3 < kChunks) fetch(tm, tn, mt, c + 3, ahead[kAhead - 1]);
+        }
+        if (EPI && mt + 1 < MT) {
+          fetch(tm, tn, mt + 1, 0, ahead[0]);
+          if (kChunks > 1) fetch(tm, tn, mt + 1, 1, ahead[kAhead - 1]);
         }
       }
       tc_fence_before();
