@@ -37,9 +37,9 @@
 // GEMMs.
 //
 // What bounds it: the instructions that turn codes into operands.  With the products left out the two kernels move
-// the weights of 4 tokens, 2 of 8 experts, 4096 x 14336 in 82 + 36 us, with the loads left out they compute for
-// 103 + 49 us, together they take 118 + 54 us (floor at the copy bandwidth 83 us); 32 tokens, 8 of 64 experts, 4096 x
-// 1376: 131 + 83 us (floor 92 us); 1 token, 8 of 64, 2048 x 1024: 21 us, of which 9 are launches, routing and fills.
+// the weights of 4 tokens, 2 of 8 experts, 4096 x 14336 in 79 + 37 us, with the loads left out they compute for
+// 105 + 50 us, together they take 108 + 54 us (floor at the copy bandwidth 83 us); 32 tokens, 8 of 64 experts, 4096 x
+// 1376: 120 + 81 us (floor 92 us); 1 token, 8 of 64, 2048 x 1024: 21 us, of which 9 are launches, routing and fills.
 // Measured and left: register double buffers (a third of the bandwidth: waiting for one step's loads waits for the
 // next step's too); a ring of each warp's own (80-110 more instructions a step: 185 us for the first case, 206 for the
 // second); 32 consumer warps of 64 registers (spills: 242 and 366 us); 16 warps that fetch in turn (190 and 234 us).

@@ -74,7 +74,8 @@ __device__ __forceinline__ Part merge(const Part& a, const Part& b) {
 template <typename T>
 struct Tile {
   static constexpr int EPV = 16 / (int)sizeof(T);
-  static constexpr uint32_t kMasked = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  static constexpr uint32_t kMasked =  // -inf, or two
+      sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
   struct alignas(16) Vec { T e[EPV]; };
 };
 
@@ -131,8 +132,9 @@ __device__ __forceinline__ float largest(const Tile<__nv_bfloat16>::Vec& q) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
-// Adds N vectors to a part.  CLAMP: any of them may be masked.  Otherwise the product e * d is 0 * -inf = NaN for a masked (-inf) element; such a tile (u is NaN,
-// s is not) is summed again with d clamped, so that the others pay nothing.
+// Adds N vectors to a part.  CLAMP: d of a masked (-inf) element is raised to -1e20, its e is 0.  Otherwise the product
+// e * d of one is 0 * -inf = NaN; such a tile (u is NaN, s is not) is summed again with d clamped, so that the others pay
+// nothing.
 template <typename T, int N, bool CLAMP>
 __device__ __forceinline__ void add_vectors(Part& p, const typename Tile<T>::Vec (&q)[N]) {
   constexpr int PAIRS = Tile<T>::EPV / 2;
@@ -271,8 +273,8 @@ __device__ void select_by_bisection(const T* __restrict__ row, int first, int la
   __syncthreads();
 }
 
-// Six CTAs on an SM with many rows: what hides the loads is occupancy (4096 x 128000 bf16: 187 us, 5.6 TB/s; four CTAs with four loads
-// per tile 194 us, three with the next tile prefetched into registers 249 us).
+// Six CTAs on an SM with many rows: what hides the loads is occupancy (4096 x 128000 bf16: 187 us, 5.6 TB/s; four CTAs
+// with four loads per tile 194 us, three with the next tile prefetched into registers 249 us).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 6)
 token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ targets, int top_n,
