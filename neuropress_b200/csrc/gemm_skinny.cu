@@ -8,9 +8,6 @@
 // no workspace, no atomics, the same bits every time.  (Reading the peers' sums instead took 9 us of 39 at 201 x 4096 x
 // 14336, a DSMEM round trip per addend; the push and the local sum take 5 of 33.)
 //
-// With more than 160 rows and many tiles two CTAs pair up on 256 outputs (cta_group::2): each loads its 128 rows of W
-// and half of the rows of x, so x crosses from L2 once per 256 outputs.
-//
 // CTA: warp 0 TMA producer (stages of 64 or 128 of k: 64-wide boxes of W and of x, 128-byte swizzle), warp 1 TMEM owner
 // and tcgen05.mma issuer, both by an elected lane of a converged warp; then all eight warps move the accumulator (TMEM
 // lane = output, column = row of x) to its shares or, unsplit, straight through the epilogue; the residual is fetched
@@ -61,7 +58,7 @@ __device__ __forceinline__ float residual_at(const SkinnyParams& p, int m, int n
   return to_f32(static_cast<const T*>(p.residual)[(int64_t)m * p.N + n]);
 }
 
-template <typename T, bool PAIR>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
 gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const SkinnyParams p) {
@@ -73,13 +70,11 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* ring = smem + kHead;
-  constexpr int CG = PAIR ? 2 : 1;
-  const int x_box = p.rows / CG * 128, stage_bytes = p.boxes * (kWBox + x_box);
+  const int x_box = p.rows * 128, stage_bytes = p.boxes * (kWBox + x_box);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int cta = PAIR || p.split > 1 ? (int)cluster_ctarank() : 0;
-  const int rank = cta / CG, side = cta % CG;  // share of K; half of the pair
-  const int n0 = (blockIdx.x / (CG * p.split) * CG + side) * BN, m0 = blockIdx.y * p.rows;
+  const int rank = p.split > 1 ? (int)cluster_ctarank() : 0;  // share of K
+  const int n0 = blockIdx.x / p.split * BN, m0 = blockIdx.y * p.rows;
   const int kb0 = (int)((int64_t)p.k_stages * rank / p.split), kb1 = (int)((int64_t)p.k_stages * (rank + 1) / p.split);
   const uint32_t tmem_cols = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : p.rows <= 128 ? 128 : 256;
 
@@ -95,21 +90,11 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tma_prefetch_desc(&map_x);
   }
   if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(tmem_slot, tmem_cols);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(tmem_slot, tmem_cols);
-      tmem_relinquish();
-    }
+    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_relinquish();
   }
   tc_fence_before();
-  if (PAIR) {
-    __syncwarp();
-    cluster_sync_all();  // the peer's barriers exist before anything is sent to them
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (p.split > 1 && p.part_at != 0) {
@@ -127,59 +112,42 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
       if (elect_one()) {
         uint8_t* st = ring + (size_t)s * stage_bytes;
-        // all bytes of a pair's stage are credited to its even CTA's barrier
-        if (side == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * stage_bytes));
+        mbar_arrive_expect_tx(&full[s], (uint32_t)stage_bytes);
         for (int h = 0; h < p.boxes; ++h) {
           const int k = (kb * p.boxes + h) * 64;
-          if (PAIR) {
-            const uint32_t bar = map_to_cta(smem_u32(&full[s]), cta & ~1);
-            tma_load_2d_pair(st + h * kWBox, &map_w, bar, k, n0);
-            tma_load_2d_pair(st + p.boxes * kWBox + h * x_box, &map_x, bar, k, m0 + side * (p.rows / 2));
-          } else {
-            tma_load_2d(st + h * kWBox, &map_w, &full[s], k, n0);
-            tma_load_2d(st + p.boxes * kWBox + h * x_box, &map_x, &full[s], k, m0);
-          }
+          tma_load_2d(st + h * kWBox, &map_w, &full[s], k, n0);
+          tma_load_2d(st + p.boxes * kWBox + h * x_box, &map_x, &full[s], k, m0);
         }
       }
       __syncwarp();
       if (++s == p.stages) { s = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
-    if (side == 0) {
-      const uint32_t idesc = umma_idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, CG * BN, p.rows);
-      const uint32_t both = 3u << (cta & ~1);
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], ph, abort_flag, p.wait_ns))) {
-          atomicExch(&g_skinny_status, 2);
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t st = smem_u32(ring + (size_t)s * stage_bytes);
-          for (int h = 0; h < p.boxes; ++h) {
-            const uint64_t a = umma_desc_sw128(st + h * kWBox), b = umma_desc_sw128(st + p.boxes * kWBox + h * x_box);
+    const uint32_t idesc = umma_idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, BN, p.rows);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], ph, abort_flag, p.wait_ns))) {
+        atomicExch(&g_skinny_status, 2);
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t st = smem_u32(ring + (size_t)s * stage_bytes);
+        for (int h = 0; h < p.boxes; ++h) {
+          const uint64_t a = umma_desc_sw128(st + h * kWBox), b = umma_desc_sw128(st + p.boxes * kWBox + h * x_box);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t more = (kb > kb0 || h > 0 || k > 0) ? 1u : 0u;
-              if (PAIR) umma_f16_pair(tmem, a + 2 * k, b + 2 * k, idesc, more);
-              else umma_f16(tmem, a + 2 * k, b + 2 * k, idesc, more);
-            }
-          }
-          if (PAIR) umma_commit_pair(&empty[s], both);
-          else umma_commit(&empty[s]);
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem, a + 2 * k, b + 2 * k, idesc, (kb > kb0 || h > 0 || k > 0) ? 1u : 0u);
         }
-        __syncwarp();
-        if (++s == p.stages) { s = 0; ph ^= 1; }
+        umma_commit(&empty[s]);
       }
-      if (ok && elect_one()) {
-        if (PAIR) umma_commit_pair(done, both);
-        else umma_commit(done);
-      }
+      __syncwarp();
+      if (++s == p.stages) { s = 0; ph ^= 1; }
     }
+    if (ok && elect_one()) umma_commit(done);
   }
   __syncwarp();
   // Epilogue, 16 rows of x at a time: two warps share the 32 outputs of a TMEM quadrant.
@@ -255,7 +223,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tc_fence_after();
     const uint32_t part = smem_u32(ring) + p.part_at;
     Four* kept = reinterpret_cast<Four*>(ring + p.part_at + p.part_rows * BN * 4);  // [row][units]
-    const uint32_t to = map_to_cta(part + (rank * p.part_rows * share + lane_n % share) * 4, lane_n / share * CG + side);
+    const uint32_t to = map_to_cta(part + (rank * p.part_rows * share + lane_n % share) * 4, lane_n / share);
     for (int first = 0; first < rows; first += p.part_rows) {
       const int here = min(p.part_rows, rows - first);
       __syncwarp();
@@ -325,23 +293,17 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
-  if (PAIR) {
-    __syncwarp();
-    cluster_sync_all();  // nothing of the peer is touched after it left
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    if (PAIR) tmem_dealloc_pair(tmem, tmem_cols);
-    else tmem_dealloc(tmem, tmem_cols);
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 
-template <typename T, bool PAIR>
+template <typename T>
 int launch_skinny(const cudaLaunchConfig_t& cfg, const CUtensorMap& map_w, const CUtensorMap& map_x,
                   const SkinnyParams& p) {
-  auto kern = gemm_skinny_kernel<T, PAIR>;
+  auto kern = gemm_skinny_kernel<T>;
   int resident = 0;
   if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kThreads, cfg.dynamicSmemBytes, &resident)) return rc;
   if (resident < 1) return NPB_ERR_TOO_LARGE;
@@ -360,7 +322,7 @@ int resident_ctas(int cluster, int* ctas) {
   NPB_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return NPB_ERR_CUDA;
   if (cached[dev][slot] == 0) {
-    auto kern = gemm_skinny_kernel<__half, false>;
+    auto kern = gemm_skinny_kernel<__half>;
     int per_sm = 0;
     const int smem = max_dynamic_smem() / 2 + 2048;
     if (int rc = blocks_per_sm(reinterpret_cast<const void*>(kern), kThreads, smem, &per_sm)) return rc;
@@ -383,18 +345,17 @@ int resident_ctas(int cluster, int* ctas) {
   return NPB_OK;
 }
 
-// Whether this form is the faster one (this / the dense kernel, us): while tiles can be split over the SMs (256 rows, 4096 x
-// 14336: 38 / 78; 512 rows, 2048 x 8192: 24 / 50); in one wave of tiles if they are not too high (128 rows, 14336 x 4096:
-// 32 / 34; 256 rows: 43 / 41); in two waves, which the dense kernel's epilogue overlaps, with few rows (64 rows, 32000 x
-// 4096: 53 / 55; 96 rows: 58 / 55) or long sums (201 rows, 28672 x 8192: 116 / 153; 96 rows, 36864 x 8192: 108 / 109); and
-// with a few rows always (16 rows, 49152 x 4096: 72 / 76; 48 rows: 88 / 77).
-bool gemm_skinny_takes(int64_t M, int64_t N, int64_t K) {
+// Whether this form is the faster one (this / the dense kernel, us): while tiles can be split over the SMs (201 rows, 4096
+// x 14336: 34 / 58; 512 rows, 2048 x 8192: 25 / 36); in one wave of two tiles to an SM (64 rows, 14336 x 4096: 28 / 31;
+// 160 rows: 34 / 39; 201 rows, with pairs of CTAs in this form as in the dense kernel: 39 / 39); in two waves, whose
+// epilogues the dense kernel overlaps, with fewer rows (64 rows, 28672 x 8192: 89 / 90; 96 rows: 93 / 89); and with a few
+// rows always (16 rows, 49152 x 4096: 78 / 82; 64 rows: 89 / 79).
+bool gemm_skinny_takes(int64_t M, int64_t N) {
   const int64_t row_tiles = (M + 255) / 256, all = row_tiles * ((N + BN - 1) / BN);
   const int64_t rows = row_tiles ? (M + row_tiles - 1) / row_tiles : 0;
   if (all * 2 <= sm_count()) return true;
-  if (all <= sm_count()) return rows <= 208;
-  if (row_tiles > 1) return false;
-  return rows <= (all > 2 * sm_count() ? 32 : K < 8192 ? 64 : 208);
+  if (all <= sm_count()) return rows <= 160;
+  return row_tiles == 1 && rows <= (all <= 2 * sm_count() ? 64 : 32);
 }
 
 // Tiles of at most 256 rows of x; W is read once per tile of rows.
@@ -407,28 +368,23 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   p.M = (int)M; p.N = (int)N; p.act = act;
   const int row_tiles = (int)((M + 255) / 256);
   const int rows = (int)((M + row_tiles - 1) / row_tiles);
-  const int64_t tiles_1 = (N + BN - 1) / BN * row_tiles;  // of one CTA
+  const int64_t tiles = (N + BN - 1) / BN;
   const int half = max_dynamic_smem() / 2 - 1024 - 2048, whole = max_dynamic_smem() - 2048;
-  auto two_fit = [&](int x_rows) { return (half - kHead) / (kWBox + x_rows * 128) >= 3; };  // CTAs on an SM
-  // Too many tiles for a split in two, one CTA to an SM: two CTAs to an SM (128 rows, 14336 x 4096: 32 us, one to an SM
-  // 39 us), or pairs where the rows leave room for one (201 rows, 14336 x 4096: 39 us against 52 us without; 400 rows, 8192 x
-  // 8192: 57 / 69 us).  Otherwise one CTA with the whole ring is better (128 rows, 4096 x 4096: 14.8 us, two to an SM
-  // 16.3 us), and pairs cost: they need clusters of eight, on fewer SMs (201 rows, 4096 x 14336: 63 / 34 us).
-  const bool crowded = tiles_1 * 2 > sm_count(), pair = crowded && !two_fit((rows + 15) / 16 * 16);
-  const int cg = pair ? 2 : 1, step = 16 * cg;
-  p.rows = (rows + step - 1) / step * step;
+  p.rows = (rows + 15) / 16 * 16;
   p.wait_ns = wait_limit_ns();
-  const int box_bytes = kWBox + p.rows / cg * 128;  // of W and x, 64 of k
-  const int per_sm = crowded && two_fit(p.rows / cg) ? 2 : 1, room = (per_sm == 2 ? half : whole) - kHead;
+  const int box_bytes = kWBox + p.rows * 128;  // of W and x, 64 of k
+  // Too many tiles for a split in two, one CTA to an SM: two CTAs to an SM (128 rows, 14336 x 4096: 32 us, one to an SM
+  // 39 us; the dense kernel takes the rows that leave no room for two).  Otherwise one CTA with the whole ring is better
+  // (128 rows, 4096 x 4096: 14.8 us, two to an SM 16.3 us).
+  const int per_sm = tiles * row_tiles * 2 > sm_count() ? 2 : 1, room = (per_sm == 2 ? half : whole) - kHead;
   p.boxes = room / box_bytes >= 6 ? 2 : 1;
   const int stage_bytes = p.boxes * box_bytes;
   p.stages = room / stage_bytes < kMaxStages ? room / stage_bytes : kMaxStages;
   p.k_stages = (int)((K + p.boxes * 64 - 1) / (p.boxes * 64));
-  const int64_t tiles = (N + cg * BN - 1) / (cg * BN) * cg;
   p.split = 1;
-  while (p.split * cg < (pair ? 4 : 8) && p.k_stages >= p.split * 4) {
+  while (p.split < 8 && p.k_stages >= p.split * 4) {
     int room_for = 0;  // CTAs that run at once, one to an SM, in clusters of twice the size
-    if (int rc = resident_ctas(p.split * cg * 2, &room_for)) return rc;
+    if (int rc = resident_ctas(p.split * 2, &room_for)) return rc;
     // where two share an SM a tenth more than run at once is better than half as many
     const int64_t most = per_sm == 2 ? room_for * 2 * 11 / 10 : room_for;
     if (tiles * row_tiles * p.split * 2 > most) break;
@@ -436,14 +392,15 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   }
   const int ring = p.stages * stage_bytes, most_rows = (int)(M < p.rows ? M : p.rows);
   const int rest = most_rows * (BN / p.split) * 2;  // the residual's share
-  const bool behind = p.split > 1 && ring + most_rows * BN * 4 + rest <= room;  // partial sums need no wait for the ring
+  // partial sums behind the ring need no wait for it
+  const bool behind = p.split > 1 && ring + most_rows * BN * 4 + rest <= room;
   p.part_at = behind ? ring : 0;
   p.part_rows = behind ? most_rows : (ring - rest) / (BN * 4) / 32 * 32;
   const bool bf16 = dtype == NPB_BF16;
   CUtensorMap map_w, map_x;
   const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (int rc = make_tensor_map_2d(&map_w, type, 2, w, N, K, BN, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  if (int rc = make_tensor_map_2d(&map_x, type, 2, x, M, K, p.rows / cg, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tensor_map_2d(&map_x, type, 2, x, M, K, p.rows, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)row_tiles);
   cfg.blockDim = dim3(kThreads);
@@ -451,15 +408,12 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = p.split * cg;
+  attr.val.clusterDim.x = p.split;
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (bf16)
-    return pair ? launch_skinny<__nv_bfloat16, true>(cfg, map_w, map_x, p)
-                : launch_skinny<__nv_bfloat16, false>(cfg, map_w, map_x, p);
-  return pair ? launch_skinny<__half, true>(cfg, map_w, map_x, p) : launch_skinny<__half, false>(cfg, map_w, map_x, p);
+  return bf16 ? launch_skinny<__nv_bfloat16>(cfg, map_w, map_x, p) : launch_skinny<__half>(cfg, map_w, map_x, p);
 }
 
 // Reads and clears the give-up record (npb_gemm_device_status collects it).

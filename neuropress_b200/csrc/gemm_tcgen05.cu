@@ -843,7 +843,7 @@ int gemm(const void* x, const void* w, const float* bias, void* y, int64_t M, in
 }
 
 // gemm_skinny.cu
-bool gemm_skinny_takes(int64_t M, int64_t N, int64_t K);
+bool gemm_skinny_takes(int64_t M, int64_t N);
 int gemm_skinny(const void* x, const void* w, const float* bias, int act, const void* residual, void* y, int64_t M,
                 int64_t N, int64_t K, int dtype, cudaStream_t st);
 
@@ -856,7 +856,7 @@ int gemm_epilogue(const void* x, const void* w, const float* bias, int act, cons
   if (w == nullptr) return NPB_ERR_INVALID_ARG;
   if (!aligned_to(w, 16) || !aligned_to(y, 2) || !aligned_to(residual, 2) || !aligned_to(bias, 4))
     return NPB_ERR_ALIGNMENT;
-  if (gemm_skinny_takes(M, N, K)) return gemm_skinny(x, w, bias, act, residual, y, M, N, K, dtype, st);
+  if (gemm_skinny_takes(M, N)) return gemm_skinny(x, w, bias, act, residual, y, M, N, K, dtype, st);
   GemmParams p{};
   p.bias = bias;
   p.y = y;

@@ -234,15 +234,6 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
       : "memory");
 }
 
-// The same for a pair anywhere in its cluster: `ctas` has the bits of its two ranks.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t ctas) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)ctas)
-      : "memory");
-}
-
 // Each lane reads 32 consecutive fp32 columns of its own TMEM lane (32 lanes x 32 columns).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(

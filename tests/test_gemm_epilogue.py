@@ -80,7 +80,7 @@ def test_shapes(shape):
     (161, 9475, 1032), (176, 9600, 8192), (201, 12803, 4104), (208, 18432, 136), (256, 9481, 264), (256, 9216, 1096),
     (300, 8192, 520), (400, 8190, 2056), (416, 9344, 72), (30, 40000, 264), (33, 40001, 264), (201, 20000, 8200)])
 def test_many_tiles(shape):
-    """CTA pairs, two CTAs to an SM and the sizes where the forms change over, with odd and even rows of outputs."""
+    """Two CTAs to an SM, CTA pairs and the sizes where the forms change over, with odd and even rows of outputs."""
     m, n, k = shape
     x, w, b, r = make(m, n, k, torch.bfloat16, seed=m + n + k)
     y = run(x, w, b, "gelu", r)
