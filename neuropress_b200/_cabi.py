@@ -221,6 +221,7 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 # The current stream's handle without building a Stream object (0.3 us instead of 3.2 us a call).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def stream_ptr() -> int:
@@ -229,12 +230,17 @@ def stream_ptr() -> int:
     return _raw_stream(torch.cuda.current_device())
 
 
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream's handle on the device of a CUDA tensor (CUDA is up where there is one)."""
+    return stream_ptr() if _raw_stream is None else _raw_stream(t.get_device())
+
+
 _NO_SWITCH = contextlib.nullcontext()
 
 
 def on_device(device: torch.device):
-    """``torch.cuda.device(device)``, free of charge where that device is the current one."""
-    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """``torch.cuda.device(device)`` of a CUDA tensor, free of charge where that device is the current one."""
+    return _NO_SWITCH if _raw_device() == device.index else torch.cuda.device(device)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:

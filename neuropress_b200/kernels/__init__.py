@@ -472,12 +472,12 @@ def gemm_epilogue(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = 
     _cabi.require_cuda("gemm_epilogue", x, w, residual)
     lib = _cabi.load_library()
     b = _bias_f32(bias, n, x.device)
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    y = x.new_empty((m, n))
     with _cabi.on_device(x.device):
         rc = _launch("npb_gemm_epilogue", lib.npb_gemm_epilogue, x.data_ptr(), w.data_ptr(),
                      None if b is None else b.data_ptr(), _cabi.ACTIVATIONS[activation],
                      None if residual is None else residual.data_ptr(), y.data_ptr(), m, n, k,
-                     _cabi.dtype_code(x.dtype), _cabi.stream_ptr())
+                     _cabi.dtype_code(x.dtype), _cabi.stream_of(x))
     _cabi.check(rc, "gemm_epilogue")
     return y
 
@@ -646,7 +646,7 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
     x_step, l_step = h * x.element_size(), e * router_logits.element_size()
     x_at, l_at, y_at, renorm = x.data_ptr(), router_logits.data_ptr(), y.data_ptr(), int(renormalize)
     with _cabi.on_device(x.device):
-        stream, scratch = _cabi.stream_ptr(), workspace.data_ptr()
+        stream, scratch = _cabi.stream_of(x), workspace.data_ptr()
         for t0 in range(0, t, n):
             rc = _launch("npb_q_moe", lib.npb_q_moe, x_at + t0 * x_step, code, l_at + t0 * l_step, logit_code,
                          min(n, t - t0), e, h, i, *structs, top_k, renorm, scratch, size, y_at + t0 * x_step, stream)
@@ -764,11 +764,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0
     _cabi.require_cuda("token_logprobs", targets, logits if logits.is_contiguous() else logits[:1])
     lib = _cabi.load_library()
     code = _cabi.dtype_code(logits.dtype)
-    logprob, entropy = logits.new_empty((r,), dtype=torch.float32), logits.new_empty((r,), dtype=torch.float32)
-    top, ids = logits.new_empty((r, top_n), dtype=torch.float32), targets.new_empty((r, top_n))
+    logprob = logits.new_empty((r,), dtype=torch.float32)
+    entropy, top, ids = logprob.new_empty((r,)), logprob.new_empty((r, top_n)), targets.new_empty((r, top_n))
     with _cabi.on_device(logits.device):
         rc = _launch("npb_token_logprobs", lib.npb_token_logprobs, logits.data_ptr(), logits.stride(0) if r > 1 else v,
                      r, v, code, targets.data_ptr(), int(top_n), logprob.data_ptr(), entropy.data_ptr(),
-                     top.data_ptr(), ids.data_ptr(), _cabi.stream_ptr())
+                     top.data_ptr(), ids.data_ptr(), _cabi.stream_of(logits))
     _cabi.check(rc, "token_logprobs")
     return logprob, entropy, top, ids
