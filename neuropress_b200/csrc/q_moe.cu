@@ -36,10 +36,10 @@
 // sum has a fixed order: results do not depend on scheduling.  Waits on the barriers are bounded like those of the
 // GEMMs.
 //
-// What bounds it: the instructions that turn codes into operands.  With the products left out the two kernels move
-// the weights of 4 tokens, 2 of 8 experts, 4096 x 14336 in 79 + 37 us, with the loads left out they compute for
-// 105 + 50 us, together they take 108 + 54 us (floor at the copy bandwidth 83 us); 32 tokens, 8 of 64 experts, 4096 x
-// 1376: 120 + 81 us (floor 92 us); 1 token, 8 of 64, 2048 x 1024: 21 us, of which 9 are launches, routing and fills.
+// What bounds it: the instructions that turn codes into operands.  4 tokens, 2 of 8 experts, 4096 x 14336: 106 + 54 us
+// cold, 151 us in a graph (floor at the copy bandwidth 83 us; without the products 79 + 36 us, without the loads 101 + 49
+// us); 32 tokens, 8 of 64 experts, 4096 x 1376: 120 + 76 us, 183 us in a graph (floor 92 us); 1 token, 8 of 64, 2048 x
+// 1024: 21 us, of which 9 are launches, routing and fills.
 // Measured and left: register double buffers (a third of the bandwidth: waiting for one step's loads waits for the
 // next step's too); a ring of each warp's own (80-110 more instructions a step: 185 us for the first case, 206 for the
 // second); 32 consumer warps of 64 registers (spills: 242 and 366 us); 16 warps that fetch in turn (190 and 234 us).
@@ -235,8 +235,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 enum { kAny = 0, kOnePerBlock = 1, kPowerOfTwo = 2 };
 
 constexpr int kConsumers = 16;                    // warps
-// Producer warps: one issues TMA, all copy the windows that TMA cannot take (four against one: 111 -> 83 us for 32 tokens
-// of 64 experts 4096 x 1376; without windows to copy the three would only cost, 118 -> 126 us for 4096 -> 14336).
+// Producer warps: one issues TMA, all copy the windows that TMA cannot take (four against one: 111 -> 83 us for 32
+// tokens of 64 experts 4096 x 1376; without windows to copy the three would only cost, 118 -> 126 us for 4096 -> 14336).
 constexpr int producers(int mode) { return mode == kAny ? 4 : 1; }
 constexpr int threads_of(int mode) { return (kConsumers + producers(mode)) * 32; }
 constexpr int kMaxStages = 4;
@@ -452,10 +452,10 @@ constexpr int kUpCodes = kUpSlices * 2 * kUpRows * 64;  // [slice][gate, up][32]
 
 // Shared memory of kernel 1 behind the routing: the ring (codes, then windows [scales of gate, of up, zero points of
 // either][32][window]), tokens [NT][4 * steps] blocks of 64 bytes (neighbouring rows in the other half of the banks),
-// their m [NT / 2][blocks + 1] (pairs in different banks) and s2 [NT / 2][blocks], 256 bytes of zeros, barriers.  The
-// partial products of an item [slice][gate, up][NT][32] take the place of the codes of its last round.
+// their m [NT / 2][blocks + 1] (pairs in different banks) and s2 [NT / 2][blocks], the partial products of two items
+// [slice][gate, up][NT][32] (while one is finished the next is computed), 256 bytes of zeros, barriers.
 struct UpLayout {
-  int windows, window_stage, x, row, m, s2, zeros, bars, bytes;
+  int windows, window_stage, x, row, m, s2, red, red_item, zeros, bars, bytes;
   __host__ __device__ UpLayout(int n_blk, int nt, bool asym, int window, int stages) {
     const int blocks = (n_blk + 3) / 4 * 4;
     windows = stages * kUpCodes;
@@ -464,7 +464,9 @@ struct UpLayout {
     row = blocks * 64 + 64;
     m = x + row * nt;
     s2 = m + nt / 2 * (blocks + 1) * 16;
-    zeros = s2 + (asym ? nt / 2 * blocks * 8 : 0);
+    red = s2 + (asym ? nt / 2 * blocks * 8 : 0);
+    red_item = kUpSlices * 2 * nt * kUpRows * 4;
+    zeros = red + 2 * red_item;
     bars = zeros + 256;
     bytes = bars + 2 * kMaxStages * 8 + 1024;  // + alignment of the start
   }
@@ -670,8 +672,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
         stage_tokens(false);
       }
       float acc[2][4] = {};
-      for (int round = 0; round < rounds; ++round) {
-        if (round > 0) advance();
+      for (int round = 0; round < rounds; ++round, advance()) {
         const int s = round * kUpSlices + ks;
         ok = sm100::mbar_wait_bounded(&full[stage], parity, &abort_flag, p.wait_ns) && ok;
         if (s < n_steps) {
@@ -684,13 +685,10 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
               acc, here, start, place, operand + s * operand_step,
               Sides{sides.m + s * 64, nullptr, sides.s2 + s * 32}, g, t, s, n_blk, p.gate);
         }
-        if (round < rounds - 1) {
-          __syncwarp();
-          if (lane == 0) sm100::mbar_arrive(&empty[stage]);
-        }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&empty[stage]);
       }
-      consumer_barrier();  // the last round's codes are read
-      float* red = reinterpret_cast<float*>(dyn + stage * kUpCodes);
+      float* red = reinterpret_cast<float*>(dyn + at.red + (item & 1) * at.red_item);
       // the blocks of a set, then the slices of K
       float* part = red + ks * 2 * NT * kUpRows;
 #pragma unroll
@@ -703,19 +701,21 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
             if (t < 4 / G) part[(w * NT + 2 * t + c) * kUpRows + mt * 16 + row_of<G>(g) + h * 8] = q;
           }
       consumer_barrier();
+      // a warp per column, a lane per row; the warps take turns, as the others go on
+      const int column = (warp - item * NT) & (kConsumers - 1);
       uint32_t m = staged;
-      for (int i = 0; i < warp; ++i) m &= m - 1;
-      const int token = __ffs(m) - 1;  // a warp per column, a lane per row
-      if (warp < NT && token >= 0 && (mask >> token & 1)) {
+      for (int i = 0; i < column; ++i) m &= m - 1;
+      const int token = __ffs(m) - 1;
+      if (column < NT && token >= 0 && (mask >> token & 1)) {
         float gate = 0.f, up = 0.f;
 #pragma unroll
         for (int k = 0; k < kUpSlices; ++k) {
-          const float* from = red + (k * 2 * NT + warp) * kUpRows + lane;
+          const float* from = red + (k * 2 * NT + column) * kUpRows + lane;
           gate += from[0];
           up += from[NT * kUpRows];
         }
-        gate *= x_f[warp];
-        up *= x_f[warp];
+        gate *= x_f[column];
+        up *= x_f[column];
         const bool chosen = lane < p.top_k && r.id[token][lane] == e;
         const int j = __ffs(__ballot_sync(0xffffffffu, chosen)) - 1;
         const float h = r.weight[token][j] * (gate / (1.f + expf(-gate)) * up);
@@ -740,10 +740,6 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
             if (lane < 4) reinterpret_cast<float*>(rec + 128)[side + lane * 2] = 0.f;
           }
       }
-      sm100::fence_proxy_async_smem();  // TMA writes there next
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&empty[stage]);
-      advance();
     }
   }
   if (!ok) {
@@ -757,11 +753,10 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
 // A CTA has 512 / slices rows of the output, 32 to each of 16 / slices warps side by side, and takes a share of the
 // (unit, round) pairs of its cluster.
 // Shared memory of kernel 2 behind the lists: the ring (codes [slice][rows][64], then windows [scales, zero points]
-// [rows][window], then h records [NT / 2][4 * slices], pairs in different banks), the sums [T][rows], zeros that
-// cover the reach of a step's operands, barriers.  The partial products of a unit [slice][NT][rows] take the place of the codes
-// of its last round.
+// [rows][window], then h records [NT / 2][4 * slices], pairs in different banks), the sums [T][rows], the
+// partial products of two units [slice][NT][rows], zeros that cover the reach of a step's operands, barriers.
 struct DownLayout {
-  int rows, windows, window_stage, h, h_pair, h_stage, sums, zeros, bars, bytes;
+  int rows, windows, window_stage, h, h_pair, h_stage, sums, red, red_unit, zeros, bars, bytes;
   __host__ __device__ DownLayout(int T, int nt, bool asym, int window, int slices, int stages) {
     rows = 512 / slices;
     windows = stages * 512 * 64;
@@ -770,7 +765,9 @@ struct DownLayout {
     h_pair = 4 * slices * kRecord + 32;
     h_stage = nt / 2 * h_pair;
     sums = h + stages * h_stage;
-    zeros = sums + T * rows * 4;
+    red = sums + T * rows * 4;
+    red_unit = 512 * nt * 4;
+    zeros = red + 2 * red_unit;
     bars = zeros + 4 * kRecord;
     bytes = bars + 2 * kMaxStages * 8 + 1024;
   }
@@ -900,10 +897,11 @@ moe_down_kernel(const __grid_constant__ DownMaps maps, const MoeParams p) {
             acc, here, start, place, operand + stage * operand_stage, Sides{side, side + 16, side + 24}, g, t, s, n_blk,
             p.down);
       }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&empty[stage]);
       if (round == rounds - 1 || q == last - 1) {
         // the unit (or this CTA's share of it) is done: its slices of k, and its tokens into the sums
-        consumer_barrier();  // the round's codes are read
-        float* red = reinterpret_cast<float*>(dyn + stage * 512 * 64);
+        float* red = reinterpret_cast<float*>(dyn + at.red + (u & 1) * at.red_unit);
         float* part = red + ks * NT * rows + r0;
 #pragma unroll
         for (int w = 0; w < 2; ++w)
@@ -918,18 +916,16 @@ moe_down_kernel(const __grid_constant__ DownMaps maps, const MoeParams p) {
         consumer_barrier();
         const uint32_t mask = lists.mask[u];
         const int n = __popc(mask);
-        for (int i = tid; i < n * rows; i += kConsumers * 32) {
-          const int c = i / rows, row = i - c * rows;
-          uint32_t m = mask;
-          for (int k = 0; k < c; ++k) m &= m - 1;
+        const int row = tid & (rows - 1), step = kConsumers * 32 / rows;  // rows: a power of two
+        uint32_t m = mask;
+        for (int c = tid / rows, at_c = 0; c < n; c += step) {
+          for (; at_c < c; ++at_c) m &= m - 1;
           float v = 0.f;
+#pragma unroll 4
           for (int k = 0; k < p.slices; ++k) v += red[(k * NT + c) * rows + row];
           sums[(__ffs(m) - 1) * rows + row] += v;
         }
-        sm100::fence_proxy_async_smem();  // TMA writes there next
       }
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&empty[stage]);
     }
   }
   if (!ok) {
