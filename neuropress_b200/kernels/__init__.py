@@ -16,6 +16,7 @@ reference's plain form.
 from __future__ import annotations
 
 import ctypes
+import functools
 import logging
 import os
 
@@ -593,6 +594,11 @@ def q_linear(x: torch.Tensor, w_pack: torch.Tensor, scale: torch.Tensor, nbits: 
 # ---------------------------------------------------------------------------
 
 
+@functools.lru_cache(maxsize=256)
+def _moe_workspace_bytes(tokens: int, top_k: int, i: int) -> int:
+    return _cabi.load_library().npb_q_moe_workspace_bytes(tokens, top_k, i)
+
+
 def _moe_weight(name: str, weight: tuple, shape: tuple, group_size: int):
     codes, scale, zero_point = weight
     if codes.shape != shape:
@@ -641,8 +647,8 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
     if t == 0:
         return y
     n = min(t, _cabi.MOE_MAX_TOKENS)
-    size = lib.npb_q_moe_workspace_bytes(n, top_k, i)
-    workspace = x.new_empty((size,), dtype=torch.uint8)
+    size = _moe_workspace_bytes(n, top_k, i)
+    workspace = x.new_empty((size // x.element_size(),))
     x_step, l_step = h * x.element_size(), e * router_logits.element_size()
     x_at, l_at, y_at, renorm = x.data_ptr(), router_logits.data_ptr(), y.data_ptr(), int(renormalize)
     with _cabi.on_device(x.device):
