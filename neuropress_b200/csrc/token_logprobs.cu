@@ -365,19 +365,34 @@ token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int
         if (pos < kListCap) sh.list[pos] = full_key(k, index);
       }
     };
-    for (int w = tid; w < n_hot * per; w += kThreads) {
-      const int h = sh.hot[w / per], i = w % per;
-      if (i == per - 1) {
-        if (rank == 0) {
-          const int o = h < head ? h : tail + h - head;
-          if (o < V && (h < head || h - head < V - tail)) offer(to_f32(row[o]), o);
-        }
-      } else if (v0 + h + i * kThreads < v1) {
-        const int at = head + (v0 + h + i * kThreads) * EPV;
-        const typename Tile<T>::Vec q = load_vec(row + at);
+    // loads in flight: four for fp32 (300 x 128000: 42 us, one 48 us), whose rows have twice the vectors; 16-bit rows lose
+    // (300 x 128000: 33 / 31 us), and with many rows the other CTAs hide the load
+    constexpr int kBatch = WIDE && sizeof(T) == 4 ? 4 : 1;
+    for (int w0 = tid; w0 < n_hot * per; w0 += kBatch * kThreads) {
+      typename Tile<T>::Vec q[kBatch];
+      int at[kBatch];
 #pragma unroll
-        for (int e = 0; e < EPV; ++e) offer(to_f32(q.e[e]), at + e);
+      for (int b = 0; b < kBatch; ++b) {
+        const int w = w0 + b * kThreads;
+        at[b] = -1;
+        if (w >= n_hot * per) continue;
+        const int h = sh.hot[w / per], i = w % per;
+        if (i == per - 1) {
+          if (rank == 0) {
+            const int o = h < head ? h : tail + h - head;
+            if (o < V && (h < head || h - head < V - tail)) offer(to_f32(row[o]), o);
+          }
+        } else if (v0 + h + i * kThreads < v1) {
+          at[b] = head + (v0 + h + i * kThreads) * EPV;
+          q[b] = load_vec(row + at[b]);
+        }
       }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (at[b] >= 0) {
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) offer(to_f32(q[b].e[e]), at[b] + e);
+        }
     }
     __syncthreads();
     if (sh.n_list > kListCap || sh.n_list < need) {
