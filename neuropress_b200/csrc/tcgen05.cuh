@@ -66,9 +66,8 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-// True for one lane of a converged warp.  The compiler knows that it is one: operands of TMA and tcgen05 instructions
-// behind it go to uniform registers directly, where a test of the lane number costs a loop over the lanes each
-// (an issuing thread spent 400 cycles on four MMAs and 500 on two loads).
+// True for one lane of a converged warp.  TMA and tcgen05 instructions belong behind it: behind a test of the lane
+// number an issuing thread spent 400 cycles on four MMAs and their commit and 500 on two loads, behind this a few.
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
   asm volatile(
