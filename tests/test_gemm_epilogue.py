@@ -78,7 +78,8 @@ def test_shapes(shape):
 @pytest.mark.parametrize("shape", [
     (1, 9601, 264), (3, 19200, 136), (33, 9480, 4104), (100, 9601, 520), (128, 18944, 264), (150, 12801, 2056),
     (161, 9475, 1032), (176, 9600, 8192), (201, 12803, 4104), (208, 18432, 136), (256, 9481, 264), (256, 9216, 1096),
-    (300, 8192, 520), (400, 8190, 2056), (416, 9344, 72), (30, 40000, 264), (33, 40001, 264), (201, 20000, 8200)])
+    (300, 8192, 520), (400, 8190, 2056), (416, 9344, 72), (30, 40000, 264), (33, 40001, 264), (201, 20000, 8200),
+    (9000, 130, 264), (18689, 100, 72)])
 def test_many_tiles(shape):
     """Two CTAs to an SM, CTA pairs and the sizes where the forms change over, with odd and even rows of outputs."""
     m, n, k = shape

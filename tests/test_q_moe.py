@@ -100,6 +100,25 @@ def test_matches_plain_implementation(t, e, k, h, i, g, asym, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("t,e,k,h,i,g", [
+    (32, 2, 1, 16384, 64, 32), (7, 2, 2, 64, 16384, 32), (8, 2, 1, 16352, 224, 224), (1, 3, 2, 16352, 32, 32),
+    (32, 2, 1, 4096, 16352, 32), (3, 2, 1, 8192, 2080, 32), (32, 1, 1, 16384, 2048, 2048),
+])
+def test_widest(t, e, k, h, i, g, asym):
+    """The ends of the range, where tokens and rings compete for shared memory and units get smaller."""
+    ex = Experts(e, h, i, g, asym, seed=h + i)
+    x, logits = ex.inputs(t, torch.bfloat16)
+    if h * i > 1 << 24:                              # some tokens of the largest, each of them on its own
+        y = run(ex, x, logits, k)
+        some = torch.tensor([0, t - 1])
+        assert_close(y[some], plain(ex, x[some], logits[some], k, True), torch.bfloat16)
+    else:
+        assert_close(run(ex, x, logits, k), plain(ex, x, logits, k, True), torch.bfloat16)
+    assert _cabi.gemm_device_status() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", [33, 70])
 def test_more_tokens_than_a_call_takes(t):
     ex = Experts(6, 128, 96, 32, False, seed=t)
