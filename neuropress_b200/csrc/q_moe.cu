@@ -36,8 +36,8 @@
 // sum has a fixed order: results do not depend on scheduling.  Waits on the barriers are bounded like those of the
 // GEMMs.
 //
-// What bounds it: the instructions that turn codes into operands.  4 tokens, 2 of 8 experts, 4096 x 14336: 106 + 54 us
-// cold, 151 us in a graph (floor at the copy bandwidth 83 us; without the products 79 + 36 us, without the loads 101 + 49
+// What bounds it: the instructions that turn codes into operands.  4 tokens, 2 of 8 experts, 4096 x 14336: 103 + 52 us
+// cold, 146 us in a graph (floor at the copy bandwidth 83 us; without the products 79 + 36 us, without the loads 101 + 49
 // us); 32 tokens, 8 of 64 experts, 4096 x 1376: 120 + 76 us, 183 us in a graph (floor 92 us); 1 token, 8 of 64, 2048 x
 // 1024: 21 us, of which 9 are launches, routing and fills.
 // Measured and left: register double buffers (a third of the bandwidth: waiting for one step's loads waits for the
@@ -372,6 +372,24 @@ __device__ __forceinline__ void add_step(float (&acc)[2][4], const StepAt& at, i
           zp[ASYM ? i : 0][h] = *reinterpret_cast<const uint2*>(from + i * at.window_tile + h * 8 * at.pitch + at.zeros);
       }
   }
+  // kPowerOfTwo: a step has one group or (64-wide) two; in the halves of a word the groups of the first and the second
+  // two blocks, or this lane's twice
+  uint32_t sw[MODE == kPowerOfTwo ? 2 : 1][2], zw[MODE == kPowerOfTwo && ASYM ? 2 : 1][2];
+  if constexpr (MODE == kPowerOfTwo) {
+    const int group = group_of(w, s * 4);
+    const uint8_t* from = row + place(group & ~1);
+    const uint32_t lower = 0x1010, upper = 0x3232;
+    const uint32_t halves = w.group_shift > 1 ? (group & 1 ? upper : lower) : G < 4 ? 0x3210 : t & 2 ? upper : lower;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* value = from + i * at.window_tile + h * 8 * at.pitch;
+        sw[i][h] = __byte_perm(*reinterpret_cast<const uint32_t*>(value), 0u, halves);
+        if (ASYM)
+          zw[ASYM ? i : 0][h] = __byte_perm(*reinterpret_cast<const uint32_t*>(value + at.zeros), 0u, halves);
+      }
+  }
 #pragma unroll
   for (int j = 0; j < 4 / G; ++j) {
     // this lane's G words of the set: 16-byte piece (block) of the row, word t mod 4 / G times G
@@ -404,7 +422,7 @@ __device__ __forceinline__ void add_step(float (&acc)[2][4], const StepAt& at, i
     // this lane's block of the set; past the row's last (whose products are zero) the last one's scale will do
     int own = s * 4 + j * G + t / (4 / G);
     if (MODE == kAny) own = min(own, n_blk - 1);
-    const uint8_t* from = MODE == kOnePerBlock ? row : row + place(group_of(w, own));
+    const uint8_t* from = MODE == kAny ? row + place(group_of(w, own)) : row;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -413,6 +431,11 @@ __device__ __forceinline__ void add_step(float (&acc)[2][4], const StepAt& at, i
         if constexpr (MODE == kOnePerBlock) {
           scale = group_value<G>(sc[q][h], j, t);
           if (ASYM) z = group_value<G>(zp[ASYM ? q : 0][h], j, t);
+        } else if constexpr (MODE == kPowerOfTwo) {
+          constexpr int kHalf = 4 / G / 2;  // sets of the first two blocks
+          const bool second = kHalf > 0 && j >= kHalf;
+          scale = half_bits(second ? sw[q][h] >> 16 : sw[q][h]);
+          if (ASYM) z = half_bits(second ? zw[ASYM ? q : 0][h] >> 16 : zw[ASYM ? q : 0][h]);
         } else {
           const uint8_t* value = from + q * at.window_tile + h * 8 * at.pitch;
           scale = half_bits(*reinterpret_cast<const uint16_t*>(value));

@@ -101,6 +101,17 @@ def test_matches_plain_implementation(t, e, k, h, i, g, asym, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("t", [1, 2, 3, 4, 20])
+@pytest.mark.parametrize("h,i,g", [(1024, 512, 64), (512, 1024, 64), (1024, 2048, 128), (2048, 2048, 256)])
+def test_groups_of_a_power_of_two(t, h, i, g, asym):
+    """Groups wider than a block in rows of whole 16-byte pieces, for every number of tokens to a product."""
+    ex = Experts(3, h, i, g, asym, seed=h + i + t)
+    x, logits = ex.inputs(t, torch.float16)
+    assert_close(run(ex, x, logits, 2), plain(ex, x, logits, 2, True), torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("asym", [False, True])
 @pytest.mark.parametrize("t,e,k,h,i,g", [
     (32, 2, 1, 16384, 64, 32), (7, 2, 2, 64, 16384, 32), (8, 2, 1, 16352, 224, 224), (1, 3, 2, 16352, 32, 32),
     (32, 2, 1, 4096, 16352, 32), (3, 2, 1, 8192, 2080, 32), (32, 1, 1, 16384, 2048, 2048),
