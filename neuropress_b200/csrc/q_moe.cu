@@ -16,9 +16,9 @@
 // codes; the activations that meet the latter are stored divided by 16.  With x' the stored activations
 //   sum_k (q - z) x = D - 1024 sum_k x' - z sum_k x,   D the mma's sum
 // is applied per 32-wide block, with the weight's scale, in fp32.  Activations are stored as fp16 after division by a
-// power of two, one per token for x and one per 32-block and token for h, so their size does not matter: x loses
-// nothing down to 2^-13 (bf16) or 2^-10 (fp16) of the token's largest and at most 2^-21 of the largest below that; h
-// keeps 11 significant bits between the kernels, 1/8 of a bf16 half step.
+// power of two that brings the largest to 2^14 (so that next to all of fp16's range lies below it), one per token for x
+// and one per 32-block and token for h.  Relative to the power of two at or below that largest, x is stored as it is down
+// to 2^-27 (bf16) or 2^-24 (fp16) and h with 11 significant bits down to 2^-24; what is smaller is off by at most 2^-35.
 //
 // The eight columns of an mma are NT = 8 / G tokens times G neighbouring 32-blocks (G = 4, 2, 1): lane (g, t)
 // of a warp loads G words, the t-th part of G blocks, of rows g and g + 8, so the k slots of an mma hold
@@ -304,10 +304,11 @@ __device__ __forceinline__ void a_operands(uint32_t l, uint32_t h, uint32_t (&a)
 }
 
 // ---- stored activations --------------------------------------------------------------------
-// The power of two at or below a magnitude (1 for zero, subnormal, inf, NaN).
-__device__ __forceinline__ float power_below(float top) {
+// The power of two that values up to a magnitude are divided by: it comes to [2^14, 2^15), which fp16 holds even where
+// its rounding goes up.  At least 2^-112, so that the product with a normal fp16 scale stays normal; 1 for inf and NaN.
+__device__ __forceinline__ float storage_power(float top) {
   const uint32_t exponent = __float_as_uint(top) >> 23;
-  return exponent == 0 || exponent == 255 ? 1.f : __uint_as_float(exponent << 23);
+  return exponent == 255 ? 1.f : __uint_as_float((exponent > 29 ? exponent - 14 : 15) << 23);
 }
 
 // A block's m and s2 from the sums of its stored values at k = 0, 2 mod 4 (`even`) and 1, 3 mod 4 (`odd`, divided
@@ -590,7 +591,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
       if (lane == 0 && i < n) atomicMax(&x_top[i], bits);
     }
     consumer_barrier();
-    if (tid < n) x_f[tid] = power_below(__uint_as_float(x_top[tid]));
+    if (tid < n) x_f[tid] = storage_power(__uint_as_float(x_top[tid]));
 #pragma unroll 1
     for (int j0 = 0; j0 < blocks * 4; j0 += kStagers) {  // whole warps
       const int j = j0 + tid;
@@ -598,7 +599,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
         if (i < n) {
-          const float by = 1.f / power_below(__uint_as_float(x_top[i]));
+          const float by = 1.f / storage_power(__uint_as_float(x_top[i]));
           uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
           float* to_m = reinterpret_cast<float*>(dyn + at.m) + (i / 2 * (blocks + 1) + (j >> 2)) * 4 + (i & 1);
           float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + (i / 2 * blocks + (j >> 2)) * 2 + (i & 1) : nullptr;
@@ -742,8 +743,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
         const bool chosen = lane < p.top_k && r.id[token][lane] == e;
         const int j = __ffs(__ballot_sync(0xffffffffu, chosen)) - 1;
         const float h = r.weight[token][j] * (gate / (1.f + expf(-gate)) * up);
-        // the power of two at or below the block's largest magnitude (1 for a block of zeros or with inf / NaN)
-        const float f = power_below(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h)))));
+        const float f = storage_power(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h)))));
         const bool is_odd = lane & 1;  // pair (lane & 3) of its word
         const __half v = __float2half_rn(h * ((is_odd ? 0.0625f : 1.f) / f));
         const float even = warp_sum(is_odd ? 0.f : __half2float(v)), odd = warp_sum(is_odd ? __half2float(v) : 0.f);
