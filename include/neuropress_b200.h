@@ -312,7 +312,13 @@ int npb_q_embedding(const int64_t* ids, int64_t T, const npb_q_weight* w, int64_
 /* A mixture-of-experts layer for up to NPB_MOE_MAX_TOKENS tokens over 4-bit group-affine experts:
  *   p = softmax(logits[t, :E]);  S = the top_k largest logits (equal logits: lowest expert)
  *   w_e = p_e, or p_e / sum_S p if renormalize
- *   y[t] = T( sum_{e in S} w_e * D_e ( silu(G_e x[t]) * (U_e x[t]) ) )          fp32 arithmetic
+ *   y[t] = T( sum_{e in S} w_e * D_e ( silu(G_e x[t]) * (U_e x[t]) ) )
+ * Routing, silu and all sums are fp32.  The values h = w_e * silu(..) * (..) go from one kernel to the
+ * other with 11 significant bits (fp16 times a power of two per 32 of them).  The products take the
+ * integer codes: a block of 32 is summed as sum (1024 + q) v - (1024 + z) sum v, then scaled; the
+ * rounding of that is about 4e-5 of the sum for codes spread over their range, and at most 2^-10 of
+ * scale * sum |v| (which shows where one value stands out and its own weights are zero).  A token with
+ * NaN or infinite x, or with h beyond fp32, yields NaN.
  * x, y [T, H] in dtype (NPB_BF16 / NPB_F16), logits [T, E] in logits_dtype (also NPB_F32).  gate / up
  * are the experts' [I, H] weights stacked to [E * I, H], down the [H, I] weights stacked to
  * [E * H, I]; nbits 4, group_size a multiple of 32, codes, scales and zero points 16-byte aligned, gate

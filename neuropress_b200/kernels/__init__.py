@@ -614,13 +614,14 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
     """A mixture-of-experts layer for a few tokens over 4-bit group-affine experts, in two kernels:
     softmax of ``router_logits`` ``[T, E]`` (fp32, bf16 or fp16), the ``top_k`` largest (equal logits:
     lowest expert; weights renormalised to sum 1 if ``renormalize``), and
-    ``y[t] = sum_e w_e * down_e(silu(gate_e(x[t])) * up_e(x[t]))`` in fp32.  ``x`` is ``[T, H]`` bf16 or
+    ``y[t] = sum_e w_e * down_e(silu(gate_e(x[t])) * up_e(x[t]))`` with fp32 sums; the values between the
+    two kernels, ``w_e * silu(..) * up_e(..)``, are held with 11 significant bits.  ``x`` is ``[T, H]`` bf16 or
     fp16; ``gate``, ``up`` and ``down`` are ``(codes, scale, zero_point or None)`` with codes
     ``[E, I, H/2]``, ``[E, I, H/2]``, ``[E, H, I/2]`` in the layout of :func:`q_linear`, scale / zero_point
     one fp16 per group of ``group_size`` (a multiple of 32).  More than 32 tokens run 32 at a time.
     An expert whose logit is ``-inf`` is not used; a token with no expert left yields zeros, one with NaN
-    or ``+inf`` logits yields NaN.  No reference counterpart (the reference runs each expert's
-    linears)."""
+    or ``+inf`` logits, or with NaN or infinite ``x``, yields NaN.  No reference counterpart
+    (the reference runs each expert's linears)."""
     if x.dim() != 2 or router_logits.dim() != 2 or router_logits.shape[0] != x.shape[0]:
         raise RuntimeError("q_moe: expected x [T, H] and router_logits [T, E].")
     if x.dtype not in (torch.float16, torch.bfloat16):

@@ -95,3 +95,21 @@ def test_one_large_channel(t, large, asym):
     weights, groups = (ex.gate, ex.up, ex.down), (32, 32, 32)
     y = run(x, logits, weights, groups, 2)
     assert excess(y, *layer(x, logits, weights, groups, 2), torch.float16, sums=1.2e-3) <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("t", [2, 4, 10])
+def test_a_token_with_an_infinity_is_nan_throughout(t, dtype, bad):
+    """Its other channels may be beyond fp16 (bf16 rows); the other tokens are as without it."""
+    ex = Experts(3, 256, 128, 32, True, seed=t)
+    x, logits = ex.inputs(t, dtype)
+    weights, groups = (ex.gate, ex.up, ex.down), (32, 32, 32)
+    good = run(x, logits, weights, groups, 2)
+    x[1, 77] = bad
+    x[1, 78] = torch.finfo(dtype).max
+    y = run(x, logits, weights, groups, 2)
+    assert bool(torch.isnan(y[1]).all())
+    keep = torch.arange(t) != 1
+    assert torch.equal(y[keep], good[keep])
