@@ -1,4 +1,5 @@
-"""How exact the mixture-of-experts layer is: tokens with one large channel, against a plain 64-bit implementation."""
+"""How exact the mixture-of-experts layer is: tokens with one large channel, a bound on the rounding of h that stays tight
+at every width, and weights of mixed forms, against a plain 64-bit implementation."""
 
 import ctypes
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 from helpers import half_ulp
-from neuropress_b200 import _cabi
+from neuropress_b200 import _cabi, kernels
 from test_q_moe import Experts, dense
 
 DEV = "cuda"
@@ -113,3 +114,56 @@ def test_a_token_with_an_infinity_is_nan_throughout(t, dtype, bad):
     assert bool(torch.isnan(y[1]).all())
     keep = torch.arange(t) != 1
     assert torch.equal(y[keep], good[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("t,e,k,h,i,g", [
+    (1, 2, 2, 64, 16384, 32), (3, 2, 1, 128, 8192, 128), (7, 3, 2, 256, 4096, 32), (32, 2, 1, 96, 2048, 32),
+    (4, 4, 2, 2048, 512, 64), (20, 8, 2, 512, 352, 32),
+])
+def test_rounding_of_h_at_every_width(t, e, k, h, i, g, asym):
+    ex = Experts(e, h, i, g if h % g == 0 else 32, asym, seed=h + i + t)
+    groups = (ex.g,) * 3
+    x, logits = ex.inputs(t, torch.float16)
+    weights = (ex.gate, ex.up, ex.down)
+    assert excess(run(x, logits, weights, groups, k), *layer(x, logits, weights, groups, k), torch.float16) <= 0
+
+
+# group sizes of gate / up and of down (rows of whole 16-byte pieces of groups or not, one block to a group or more), and
+# which of the two have zero points
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [2, 4, 13])
+@pytest.mark.parametrize("asym_up,asym_down", [(False, True), (True, False), (True, True), (False, False)])
+@pytest.mark.parametrize("g_up,g_down", [(32, 64), (64, 32), (96, 32), (32, 96), (128, 96), (96, 128), (256, 512)])
+def test_mixed_forms(g_up, g_down, asym_up, asym_down, t):
+    h, i = (768, 1536) if 96 in (g_up, g_down) else (1024, 2048)
+    up = Experts(3, h, i, g_up, asym_up, seed=g_up + t)
+    down = Experts(3, h, i, g_down, asym_down, seed=g_down + t)
+    x, logits = up.inputs(t, torch.float16)
+    weights, groups = (up.gate, up.up, down.down), (g_up, g_up, g_down)
+    assert excess(run(x, logits, weights, groups, 2), *layer(x, logits, weights, groups, 2), torch.float16) <= 0
+
+
+@pytest.mark.gpu
+def test_wrapper_takes_zero_points_in_one_place_only():
+    for asym_up in (False, True):
+        a, b = (Experts(4, 256, 128, 32, s, seed=5) for s in (asym_up, not asym_up))
+        x, logits = a.inputs(6, torch.float16)
+        weights = (a.gate, a.up, b.down)
+        on = [tuple(None if v is None else v.to(DEV) for v in w) for w in weights]
+        y = kernels.q_moe(x.to(DEV), logits.to(DEV), *on, 2, 32)
+        assert excess(y, *layer(x, logits, weights, (32, 32, 32), 2), torch.float16) <= 0
+
+
+# ---- on the CPU -----------------------------------------------------------------------------
+@pytest.mark.parametrize("i", [256, 4096])
+def test_the_bound_sees_a_loss_of_three_bits_of_h(i):
+    ex = Experts(2, 64, i, 32, False, seed=i)
+    x, logits = ex.inputs(6, torch.float16)
+    weights, groups = (ex.gate, ex.up, ex.down), (32, 32, 32)
+    ref, spread = layer(x, logits, weights, groups, 2)
+    as_stored = layer(x, logits, weights, groups, 2, torch.float16)[0].half()
+    assert excess(as_stored, ref, spread, torch.float16) <= 0
+    eight_bits = layer(x, logits, weights, groups, 2, torch.bfloat16)[0].half()
+    assert excess(eight_bits, ref, spread, torch.float16) > 0
