@@ -7,7 +7,7 @@ keeps its experts as separate linears; lowered one by one (:class:`NPLinear`) a 
 three kernels per chosen expert and needs the choice on the host.  :meth:`NPMoE.from_experts` stacks
 their packed weights -- same bytes, same layout, expert after expert -- and ``forward`` runs the router
 as it is and then ``kernels.q_moe``: no host synchronisation, so it can be captured in a CUDA graph.
-More than 32 tokens run 32 at a time.  The stacked weights are copies, and the block is not taken
+More than 32 tokens run 32 at a time.  Casting the module casts the router only.  The stacked weights are copies, and the block is not taken
 apart again by ``unlower_model``: keep the lowered experts where that is wanted.  No reference counterpart.
 """
 
@@ -82,6 +82,17 @@ class NPMoE(nn.Module):
             stacked.append((torch.stack([m.u8_blob for m in column]), torch.stack([m.scale for m in column]),
                             None if first.zero_point is None else torch.stack([m.zero_point for m in column])))
         return cls(router, *stacked, top_k, triples[0][0].group_size, renormalize)
+
+    def _apply(self, fn, recurse: bool = True):
+        """A cast of the module (``.to(torch.bfloat16)`` for the router, say) leaves the scales and zero points fp16: they
+        are part of the packed format.  They move with the device."""
+        packed = {n: b for n, b in self._buffers.items() if b is not None and b.dtype == torch.float16}
+        super()._apply(fn, recurse)
+        for name, before in packed.items():
+            after = self._buffers[name]
+            if after.dtype != torch.float16:
+                self._buffers[name] = before.to(after.device)
+        return self
 
     def _weight(self, name: str) -> tuple:
         return getattr(self, f"{name}_codes"), getattr(self, f"{name}_scale"), getattr(self, f"{name}_zero_point")
