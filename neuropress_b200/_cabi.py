@@ -22,7 +22,7 @@ NPB_F16, NPB_BF16, NPB_F32 = 0, 1, 2
 GEMV_MAX_ROWS = 8
 LOGPROBS_MAX_TOP = 32
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # npb_activation
-MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 32, 512, 16
+MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K, MOE_MAX_WIDTH = 32, 512, 16, 16384
 STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 
 _DTYPE_CODE = {torch.float16: NPB_F16, torch.bfloat16: NPB_BF16, torch.float32: NPB_F32}

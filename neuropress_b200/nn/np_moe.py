@@ -18,6 +18,7 @@ from collections.abc import Iterable
 import torch
 from torch import nn
 
+from .. import _cabi
 from .np_linear import NPLinear
 
 __all__ = ["NPMoE"]
@@ -49,8 +50,10 @@ class NPMoE(nn.Module):
         e, i, half_h = gate[0].shape
         if tuple(up[0].shape) != (e, i, half_h) or tuple(down[0].shape) != (e, 2 * half_h, i // 2):
             raise ValueError("gate and up must be [E, I, H/2], down [E, H, I/2].")
-        if not 1 <= top_k <= e:
-            raise ValueError("top_k must lie in [1, number of experts].")
+        if e > _cabi.MOE_MAX_EXPERTS or max(2 * half_h, i) > _cabi.MOE_MAX_WIDTH:
+            raise ValueError(f"at most {_cabi.MOE_MAX_EXPERTS} experts, H and I at most {_cabi.MOE_MAX_WIDTH}.")
+        if not 1 <= top_k <= min(e, _cabi.MOE_MAX_TOP_K):
+            raise ValueError(f"top_k must lie in [1, min(number of experts, {_cabi.MOE_MAX_TOP_K})].")
         if group_size % 32 or (2 * half_h) % group_size or i % group_size:
             raise ValueError("group_size must be a multiple of 32 that divides H and I.")
         if (gate[2] is None) != (up[2] is None):

@@ -1,4 +1,4 @@
-"""NPMoE as a module of a model: casts and moves."""
+"""NPMoE as a module of a model: casts, moves and the limits of its kernel."""
 
 import pytest
 import torch
@@ -47,3 +47,21 @@ def test_moved_and_cast_in_one_step_it_runs():
     x = torch.randn(5, 64, generator=torch.Generator().manual_seed(2)).to(DEV, torch.bfloat16)
     assert torch.equal(got(x), want(x))
     assert got.gate_scale.is_cuda and got.gate_scale.dtype == torch.float16
+
+
+def test_the_kernels_limits_are_checked_when_it_is_built():
+    def weight(e, rows, cols):
+        codes = torch.zeros(1, 1, 1, dtype=torch.uint8).expand(e, rows, cols // 2)
+        return codes, torch.zeros(1), None
+
+    def build(e, h, i, top_k):
+        return NPMoE(nn.Identity(), weight(e, i, h), weight(e, i, h), weight(e, h, i), top_k, 32)
+
+    assert build(32, 32, 32, 16).top_k == 16
+    with pytest.raises(ValueError, match="top_k"):
+        build(32, 32, 32, 17)
+    with pytest.raises(ValueError, match="at most 512 experts"):
+        build(513, 32, 32, 2)
+    for h, i in ((16416, 32), (32, 16416)):
+        with pytest.raises(ValueError, match="at most 16384"):
+            build(1, h, i, 1)
