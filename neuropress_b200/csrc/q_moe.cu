@@ -304,12 +304,12 @@ __device__ __forceinline__ void a_operands(uint32_t l, uint32_t h, uint32_t (&a)
 }
 
 // ---- stored activations --------------------------------------------------------------------
-// The power of two that values up to a magnitude are divided by: it comes to [2^14, 2^15), which fp16 holds even where
-// its rounding goes up.  At least 2^-112, so that the product with a normal fp16 scale stays normal; 1 for inf and NaN.
-__device__ __forceinline__ float storage_power(float top) {
-  const uint32_t exponent = __float_as_uint(top) >> 23;
-  return exponent == 255 ? 1.f : __uint_as_float((exponent > 29 ? exponent - 14 : 15) << 23);
-}
+// The power of two that values up to a magnitude are divided by, as its exponent field (15..241): the magnitude comes to
+// [2^14, 2^15), which fp16 holds even where its rounding goes up.  At least 2^-112, so that the product with a normal fp16
+// scale stays normal.  (Infinite values stay so, and their products become NaN.)
+__device__ __forceinline__ uint32_t storage_exponent(float top) { return max(__float_as_uint(top) >> 23, 29u) - 14u; }
+__device__ __forceinline__ float power_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+__device__ __forceinline__ float reciprocal_of(uint32_t exponent) { return __uint_as_float((254u - exponent) << 23); }
 
 // A block's m and s2 from the sums of its stored values at k = 0, 2 mod 4 (`even`) and 1, 3 mod 4 (`odd`, divided
 // by 16).
@@ -591,7 +591,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
       if (lane == 0 && i < n) atomicMax(&x_top[i], bits);
     }
     consumer_barrier();
-    if (tid < n) x_f[tid] = storage_power(__uint_as_float(x_top[tid]));
+    if (tid < n) x_f[tid] = power_of(storage_exponent(__uint_as_float(x_top[tid])));
 #pragma unroll 1
     for (int j0 = 0; j0 < blocks * 4; j0 += kStagers) {  // whole warps
       const int j = j0 + tid;
@@ -599,7 +599,8 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
         if (i < n) {
-          const float by = 1.f / storage_power(__uint_as_float(x_top[i]));
+          // a division (exact), not reciprocal_of: with that the compiler spills (32 tokens, 8 of 64 experts: 192 us, 188 us)
+          const float by = 1.f / power_of(storage_exponent(__uint_as_float(x_top[i])));
           uint4* to = reinterpret_cast<uint4*>(dyn + at.x + i * at.row + j * 16);
           float* to_m = reinterpret_cast<float*>(dyn + at.m) + (i / 2 * (blocks + 1) + (j >> 2)) * 4 + (i & 1);
           float* to_s2 = ASYM ? reinterpret_cast<float*>(dyn + at.s2) + (i / 2 * blocks + (j >> 2)) * 2 + (i & 1) : nullptr;
@@ -743,9 +744,9 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
         const bool chosen = lane < p.top_k && r.id[token][lane] == e;
         const int j = __ffs(__ballot_sync(0xffffffffu, chosen)) - 1;
         const float h = r.weight[token][j] * (gate / (1.f + expf(-gate)) * up);
-        const float f = storage_power(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h)))));
+        const uint32_t f = storage_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h)))));
         const bool is_odd = lane & 1;  // pair (lane & 3) of its word
-        const __half v = __float2half_rn(h * ((is_odd ? 0.0625f : 1.f) / f));
+        const __half v = __float2half_rn(h * reciprocal_of(is_odd ? f + 4u : f));
         const float even = warp_sum(is_odd ? 0.f : __half2float(v)), odd = warp_sum(is_odd ? __half2float(v) : 0.f);
         const int rank = __popc(mask & ((1u << token) - 1u)), side = rank & 1;
         const int padded = (tiles + 3) / 4 * 4;
@@ -754,7 +755,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
         if (lane == 0) {
           float* to = reinterpret_cast<float*>(rec + 128) + side;
           put_sides(to, to + 6, even, odd, p.down.zp != nullptr);
-          to[4] = f;
+          to[4] = power_of(f);
         }
         if (i0 / 32 == tiles - 1)  // zeros behind the last block, up to a whole step
           for (int i = tiles; i < padded; ++i) {
