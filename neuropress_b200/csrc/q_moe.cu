@@ -230,6 +230,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// For the producers.  A consumer whose wait gave up raises the flag, then goes on to free stages that copies may still land
+// in: those are not filled again.
+__device__ __forceinline__ bool stage_is_free(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t wait_ns) {
+  return sm100::mbar_wait_bounded(bar, parity, abort_flag, wait_ns) && *abort_flag == 0;
+}
+
 // How groups come: kOnePerBlock (a group is a block) and kPowerOfTwo (a group is 2^n blocks) have rows of whole 16-byte
 // pieces, which TMA takes; kAny is the rest.
 enum { kAny = 0, kOnePerBlock = 1, kPowerOfTwo = 2 };
@@ -643,7 +649,7 @@ moe_up_kernel(const __grid_constant__ UpMaps maps, const MoeParams p) {
     for (int item = first; item < last && ok; ++item) {
       const int u = item / tiles, row = r.units.expert[u] * p.I + (item - u * tiles) * kUpRows;
       for (int round = 0; round < rounds; ++round, advance()) {
-        ok = sm100::mbar_wait_bounded(&empty[stage], parity ^ 1, &abort_flag, p.wait_ns);
+        ok = stage_is_free(&empty[stage], parity ^ 1, &abort_flag, p.wait_ns);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -867,7 +873,7 @@ moe_down_kernel(const __grid_constant__ DownMaps maps, const MoeParams p) {
     const uint32_t base = sm100::smem_u32(dyn);
     const int64_t total_groups = (int64_t)p.E * p.H * n_group;
     for (int q = first; q < last; ++q, advance()) {
-      ok = sm100::mbar_wait_bounded(&empty[stage], parity ^ 1, &abort_flag, p.wait_ns);
+      ok = stage_is_free(&empty[stage], parity ^ 1, &abort_flag, p.wait_ns);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
