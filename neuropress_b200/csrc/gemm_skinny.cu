@@ -48,7 +48,7 @@ struct SkinnyParams {
   int rows;       // of x per tile: multiple of 16, at most 256
   int boxes;      // of 64 of k per stage: 1 or 2
   int stages, k_stages, split;
-  int part_rows;  // rows of x whose partial sums fit: in the ring, or
+  int part_rows;  // rows of x of the largest tile: their partial sums lie in the ring, or
   int part_at;    // behind it, so many bytes from its start (0: in it)
   uint64_t wait_ns;
 };
@@ -187,8 +187,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tc_fence_before();
   } else {
     // A CTA of the cluster finishes its share of the tile's outputs.  The others push their partial sums of them into
-    // its shared memory, [rank][row of x][share], as many rows of x at a time as fit; it adds them in rank order, four
-    // outputs of a row at a time.
+    // its shared memory, [rank][row of x][share]; it adds them in rank order, four outputs of a row at a time.
     struct alignas(8) Four { T e[4]; };
     constexpr int kAhead = 16;  // units of a thread, at most (256 rows, a split in two)
     const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 &&
@@ -224,67 +223,62 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t part = smem_u32(ring) + p.part_at;
     Four* kept = reinterpret_cast<Four*>(ring + p.part_at + p.part_rows * BN * 4);  // [row][units]
     const uint32_t to = map_to_cta(part + (rank * p.part_rows * share + lane_n % share) * 4, lane_n / share);
-    for (int first = 0; first < rows; first += p.part_rows) {
-      const int here = min(p.part_rows, rows - first);
-      __syncwarp();
-      if (first == 0 && p.part_at != 0) cluster_wait();  // the others have started
-      else cluster_sync_all();  // the others are through with their rings, or with the rows before
-      if (first == 0) {
-        if (tid / units < rows) kept[tid] = rest[0];
-        if (more) {
+    __syncwarp();
+    if (p.part_at != 0) cluster_wait();  // the others have started
+    else cluster_sync_all();             // the others are through with their rings
+    if (tid / units < rows) kept[tid] = rest[0];
+    if (more) {
 #pragma unroll
-          for (int j = 1; j < kAhead; ++j)
-            if (tid / units + j * row_step < rows) kept[j * kThreads + tid] = rest[j];
-        }
-      }
-      if (got) {
-        for (int c = c0; c < here; c += 32) {
-          uint32_t v[16];
-          tmem_ld_32x32_x16(acc + first + c, v);
-          tmem_ld_wait();
+      for (int j = 1; j < kAhead; ++j)
+        if (tid / units + j * row_step < rows) kept[j * kThreads + tid] = rest[j];
+    }
+    if (got) {
+      for (int c = c0; c < rows; c += 32) {
+        uint32_t v[16];
+        tmem_ld_32x32_x16(acc + c, v);
+        tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < here)
-              asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (c + i) * share * 4), "r"(v[i]) : "memory");
-        }
+        for (int i = 0; i < 16; ++i)
+          if (c + i < rows)
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (c + i) * share * 4), "r"(v[i]) : "memory");
       }
-      __syncwarp();
-      cluster_sync_all();
-      const float4* from = reinterpret_cast<const float4*>(ring + p.part_at) + tid;
+    }
+    __syncwarp();
+    cluster_sync_all();
+    const float4* from = reinterpret_cast<const float4*>(ring + p.part_at) + tid;
 #pragma unroll 1  // a short body: it runs a few times, and fetching it costs more than running it
-      for (int row = tid / units; row < here; row += 2 * row_step, from += 2 * kThreads) {
-        const bool two = row + row_step < here;
-        const int next = two ? kThreads : 0;
-        float sum[8];
+    for (int row = tid / units; row < rows; row += 2 * row_step, from += 2 * kThreads) {
+      const bool two = row + row_step < rows;
+      const int next = two ? kThreads : 0;
+      float sum[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+      for (int k = 0; k < 8; ++k) sum[k] = 0.f;
 #pragma unroll 2
-        for (int c = 0; c < p.split; ++c) {
-          const float4 q = from[c * p.part_rows * units], r = from[c * p.part_rows * units + next];
-          sum[0] += q.x; sum[1] += q.y; sum[2] += q.z; sum[3] += q.w;
-          sum[4] += r.x; sum[5] += r.y; sum[6] += r.z; sum[7] += r.w;
+      for (int c = 0; c < p.split; ++c) {
+        const float4 q = from[c * p.part_rows * units], r = from[c * p.part_rows * units + next];
+        sum[0] += q.x; sum[1] += q.y; sum[2] += q.z; sum[3] += q.w;
+        sum[4] += r.x; sum[5] += r.y; sum[6] += r.z; sum[7] += r.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += bias[k & 3];
+      activate_all(sum, p.act);
+      const Four* rest = kept + row * units + tid % units;
+      T* y = static_cast<T*>(p.y) + (int64_t)(m0 + row) * p.N + n;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Four r = rest[j * next];
+        Four f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.e[k] = from_f32<T>(sum[j * 4 + k] + to_f32(r.e[k]));
+        if (j == 1 && !two) break;
+        if (wide) {
+          if (n < p.N) *reinterpret_cast<Four*>(y) = f;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n + k < p.N) y[k] = f.e[k];
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] += bias[k & 3];
-        activate_all(sum, p.act);
-        const Four* rest = kept + (first + row) * units + tid % units;
-        T* y = static_cast<T*>(p.y) + (int64_t)(m0 + first + row) * p.N + n;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const Four r = rest[j * next];
-          Four f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) f.e[k] = from_f32<T>(sum[j * 4 + k] + to_f32(r.e[k]));
-          if (j == 1 && !two) break;
-          if (wide) {
-            if (n < p.N) *reinterpret_cast<Four*>(y) = f;
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (n + k < p.N) y[k] = f.e[k];
-          }
-          y += (int64_t)row_step * p.N;
-        }
+        y += (int64_t)row_step * p.N;
       }
     }
     tc_fence_before();
@@ -392,10 +386,13 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   }
   const int ring = p.stages * stage_bytes, most_rows = (int)(M < p.rows ? M : p.rows);
   const int rest = most_rows * (BN / p.split) * 2;  // the residual's share
-  // partial sums behind the ring need no wait for it
-  const bool behind = p.split > 1 && ring + most_rows * BN * 4 + rest <= room;
+  // partial sums behind the ring need no wait for it; in it they have room whatever the sizes are (16 rows to spare at
+  // least, with 227 KB to a CTA)
+  const int join = p.split > 1 ? most_rows * BN * 4 + rest : 0;
+  const bool behind = join > 0 && ring + join <= room;
+  if (!behind && join > ring) return NPB_ERR_TOO_LARGE;
   p.part_at = behind ? ring : 0;
-  p.part_rows = behind ? most_rows : (ring - rest) / (BN * 4) / 32 * 32;
+  p.part_rows = most_rows;
   const bool bf16 = dtype == NPB_BF16;
   CUtensorMap map_w, map_x;
   const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -404,7 +401,7 @@ int gemm_skinny(const void* x, const void* w, const float* bias, int act, const 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)row_tiles);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 1024 + kHead + ring + (behind ? most_rows * BN * 4 + rest : 0);
+  cfg.dynamicSmemBytes = 1024 + kHead + ring + (behind ? join : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
