@@ -366,7 +366,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     const int64_t col0 = gathered ? p.sink.col0 : 0;
     if (gathered) y = static_cast<T*>(p.sink.peer_out[p.sink.rank]);
     struct alignas(16) Out { T e[8]; };
-    constexpr int kChunks = BN / 32, kAhead = EPI && kChunks > 1 ? 2 : 1;  // 32 outputs of a row
+    constexpr int kChunks = BN / 32, kAhead = EPI ? 2 : 1;  // 32 outputs of a row
+    static_assert(!EPI || (MT == 1 && kChunks >= 2), "the residual's first two chunks are fetched once a tile");
     const T* res = EPI ? static_cast<const T*>(p.residual) : nullptr;
     // 16-byte accesses only where the address itself is 16-byte aligned (a tensor that is a view at an odd offset takes
     // the element-wise path)
@@ -377,8 +378,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     // The residual of a chunk is on its way while the chunk before the last one is finished, a tile's first two while
     // the tile is waited for.
     Out ahead[kAhead][4];
-    auto fetch = [&](int tm, int tn, int mt, int c, Out (&o)[4]) {
-      const int m = (tm * MT + mt) * BM + quad * 32 + lane, n0 = tn * BN + c * 32;
+    auto fetch = [&](int tm, int tn, int c, Out (&o)[4]) {
+      const int m = tm * BM + quad * 32 + lane, n0 = tn * BN + c * 32;  // MT = 1
       const int64_t off = (int64_t)m * ld + col0 + n0;
       if (res && m < p.M && n0 < p.N && whole(off, n0)) {
 #pragma unroll
@@ -395,8 +396,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       const int buf = (NBUF == 2) ? (it & 1) : 0;
       const uint32_t buf_ph = (NBUF == 2) ? ((it >> 1) & 1) : (it & 1);
       if (EPI) {
-        fetch(tm, tn, 0, 0, ahead[0]);
-        if (kChunks > 1) fetch(tm, tn, 0, 1, ahead[kAhead - 1]);
+        fetch(tm, tn, 0, ahead[0]);
+        fetch(tm, tn, 1, ahead[kAhead - 1]);
       }
       // All lanes wait (each needs the acquire), then agree on the outcome so that the
       // warp-collective tcgen05.ld below is never reached by part of a warp.
@@ -474,14 +475,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
 #pragma unroll 1
         for (int c = 0; c < kChunks; c += kAhead) {
           finish(c, ahead[0]);
-          if (EPI && c + 2 < kChunks) fetch(tm, tn, mt, c + 2, ahead[0]);
+          if (EPI && c + 2 < kChunks) fetch(tm, tn, c + 2, ahead[0]);
           if (kAhead == 1 || c + 1 == kChunks) continue;
           finish(c + 1, ahead[kAhead - 1]);
-          if (EPI && c + 3 < kChunks) fetch(tm, tn, mt, c + 3, ahead[kAhead - 1]);
-        }
-        if (EPI && mt + 1 < MT) {
-          fetch(tm, tn, mt + 1, 0, ahead[0]);
-          if (kChunks > 1) fetch(tm, tn, mt + 1, 1, ahead[kAhead - 1]);
+          if (EPI && c + 3 < kChunks) fetch(tm, tn, c + 3, ahead[kAhead - 1]);
         }
       }
       tc_fence_before();
