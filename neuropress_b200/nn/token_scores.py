@@ -27,13 +27,15 @@ class TokenScores(NamedTuple):
 def score_tokens(lm_head: nn.Module, hidden: torch.Tensor, targets: torch.Tensor, top_n: int = 0,
                  rows_per_chunk: int = 1024, vocab_size: int | None = None) -> TokenScores:
     """``hidden`` ``[..., H]`` are the states that predict ``targets`` ``[...]`` (int64; an id outside the vocabulary,
-    such as an ignore index, scores 0).  ``vocab_size`` cuts the logits of a padded lm_head."""
+    such as an ignore index, scores 0).  ``vocab_size`` cuts the logits of a padded lm_head, which must have that many."""
     from .. import kernels
 
     if hidden.dim() < 1 or hidden.shape[:-1] != targets.shape:
         raise RuntimeError("score_tokens: expected hidden [..., H] and targets [...].")
     if rows_per_chunk < 1:
         raise RuntimeError("score_tokens: rows_per_chunk must be positive.")
+    if vocab_size is not None and vocab_size < 1:
+        raise RuntimeError("score_tokens: vocab_size must be positive.")
     leading, rows = targets.shape, targets.numel()
     h2, t2 = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1).contiguous()
     if rows == 0:
@@ -44,6 +46,8 @@ def score_tokens(lm_head: nn.Module, hidden: torch.Tensor, targets: torch.Tensor
     for r in range(0, rows, rows_per_chunk):
         logits = lm_head(h2[r:r + rows_per_chunk])
         if vocab_size is not None:
+            if vocab_size > logits.shape[-1]:
+                raise RuntimeError(f"score_tokens: vocab_size is {vocab_size}, the lm_head has {logits.shape[-1]} logits.")
             logits = logits[:, :vocab_size]
         parts.append(kernels.token_logprobs(logits, t2[r:r + rows_per_chunk], top_n=top_n))
     whole = parts[0] if len(parts) == 1 else [torch.cat(p) for p in zip(*parts)]
