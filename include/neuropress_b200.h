@@ -396,10 +396,11 @@ int npb_vq_gemv_allgather(const npb_vq_weight* w, const void* x, int x_dtype, in
                           const npb_gather_sink* sink, npb_stream_t stream);
 
 
-/* Every wait inside the tensor-core GEMMs (on an mbarrier) is bounded; a kernel that gives up
- * records which role did so, frees its tensor memory and returns.  This call synchronises the
- * device, copies that record to *host_out (0 = no give-up since the last call), clears it, and
- * returns NPB_ERR_DEVICE_TIMEOUT if it was set.  No reference counterpart. */
+/* Every wait inside the tensor-core GEMMs and npb_q_moe (on an mbarrier) is bounded; a kernel that
+ * gives up records it, frees the tensor memory it holds and returns.  This call synchronises the
+ * device, copies that record to *host_out (0 = no give-up since the last call; 50 + kernel, 1 or 2, for
+ * npb_q_moe; 60 + role for the few-row form of npb_gemm_epilogue; other values are roles of the other
+ * GEMMs), clears it, and returns NPB_ERR_DEVICE_TIMEOUT if it was set.  No reference counterpart. */
 int npb_gemm_device_status(int* host_out);
 
 /* Limit of every bounded in-kernel wait of this library (the mbarrier waits of the GEMMs, the

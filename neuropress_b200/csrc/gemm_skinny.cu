@@ -1,12 +1,14 @@
-// Dense GEMM with epilogue for few rows of x:  y[M, N] = T( act(x W^T + bias) + residual ),  M up to a few hundred.
+// Dense GEMM with epilogue for products of few tiles:  y[M, N] = T( act(x W^T + bias) + residual ).  That is few rows, up to
+// a few hundred, or any number of rows with so few outputs that the tiles fill at most half of the SMs
+// (gemm_skinny_takes).
 //
 // With few rows the product is bound by the one read of W, and the dense kernel (gemm_tcgen05.cu) has too few
 // tiles for it: 128 rows of x by up to 256 of W leave most SMs idle at N = 4096.  Here W is the 128-row operand
 // of tcgen05.mma and the rows of x are its columns (16..256, as many as there are), so a tile is 128 outputs wide
 // whatever M is, and K is split over a cluster of 1..8 CTAs, which puts every SM to work.  Each CTA finishes a share of
 // the tile's outputs: the others push their partial sums of them into its shared memory, it adds them in rank order --
-// no workspace, no atomics, the same bits every time.  (Reading the peers' sums instead took 9 us of 39 at 201 x 4096 x
-// 14336, a DSMEM round trip per addend; the push and the local sum take 5 of 33.)
+// no workspace, no atomics, the same bits every time.  (Reading the peers' sums instead is a DSMEM round trip per addend:
+// 201 x 4096 x 14336 took 39 us with it, 33 with the push.)
 //
 // CTA: warp 0 TMA producer (stages of 64 or 128 of k: 64-wide boxes of W and of x, 128-byte swizzle), warp 1 TMEM owner
 // and tcgen05.mma issuer, both by an elected lane of a converged warp; then all eight warps move the accumulator (TMEM
@@ -14,8 +16,8 @@
 // before the sums are there.  Up to two CTAs share an SM.  Every wait is bounded (npb_set_wait_limit_ns); on give-up
 // the kernel records it, lets its copies land, frees its TMEM and returns.
 //
-// 1 x 4096 x 4096: 10.6 us (floor at the copy bandwidth 5.1), 16 x 14336 x 4096: 24.4 us (18.0), 201 x 4096 x 14336:
-// 32.7 us (19.3; 10 TB/s into the SMs).
+// In a CUDA graph (launched one by one in brackets): 1 x 4096 x 4096 10.3 us (10.9; floor at the copy bandwidth 5.1), 16 x
+// 14336 x 4096 25.7 us (26.6; 18.0), 201 x 4096 x 14336 34.0 us (37.5; 19.3; 9 TB/s into the SMs).
 #include <type_traits>
 
 #include "activation.cuh"

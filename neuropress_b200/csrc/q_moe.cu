@@ -36,10 +36,14 @@
 // sum has a fixed order: results do not depend on scheduling.  Waits on the barriers are bounded like those of the
 // GEMMs.
 //
-// What bounds it: the instructions that turn codes into operands.  4 tokens, 2 of 8 experts, 4096 x 14336: 103 + 52 us
-// cold, 146 us in a graph (floor at the copy bandwidth 83 us; without the products 79 + 36 us, without the loads 101 + 49
-// us); 32 tokens, 8 of 64 experts, 4096 x 1376: 120 + 76 us, 183 us in a graph (floor 92 us); 1 token, 8 of 64, 2048 x
-// 1024: 21 us, of which 9 are launches, routing and fills.
+// What bounds it: the consumers' own latency.  Without the loads the two kernels take 101 + 49 us of 103 + 52 (4 tokens, 2 of
+// 8 experts, 4096 x 14336), without the products 79 + 36, so the products are the longer part; but they use 54-60 % of the
+// issue slots (about 300 instructions a step: 16 mma.sync, 80 that turn codes into operands), and their largest stall is
+// the fixed-latency wait: four warps a scheduler with one chain each do not cover it.  Most forms of kernel 1 spill a few
+// registers at 96 (up to 150 bytes a thread).  In a CUDA graph: that case 152 us (floor at the copy bandwidth 83), 32
+// tokens, 8 of 64 experts, 4096 x 1376 188 us (92), 1 token, 8 of 64, 2048 x 1024 21 us, of which 9 are launches, routing and
+// fills.  More than 32 tokens take a pair of launches for every 32, which read and convert their experts again: 512 tokens of
+// 4096 x 1376 3.0 ms, 2048 12 ms (expert by expert through the framework's 4-bit linears 4.5 and 5.1 ms).
 // Measured and left: register double buffers (a third of the bandwidth: waiting for one step's loads waits for the
 // next step's too); a ring of each warp's own (80-110 more instructions a step: 185 us for the first case, 206 for the
 // second); 32 consumer warps of 64 registers (spills: 242 and 366 us); 16 warps that fetch in turn (190 and 234 us).

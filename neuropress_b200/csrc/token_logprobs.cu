@@ -273,8 +273,9 @@ __device__ void select_by_bisection(const T* __restrict__ row, int first, int la
   __syncthreads();
 }
 
-// Six CTAs on an SM with many rows: what hides the loads is occupancy (4096 x 128000 bf16: 187 us, 5.6 TB/s; four CTAs
-// with four loads per tile 194 us, three with the next tile prefetched into registers 249 us).
+// Six CTAs on an SM with many rows: what hides the loads is occupancy (4096 x 128000 bf16 in a CUDA graph: 187 us, 5.6
+// TB/s, launched one by one 214-219 us; four CTAs with four loads per tile 194 us, three with the next tile prefetched into
+// registers 249 us).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 6)
 token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ targets, int top_n,

@@ -618,7 +618,9 @@ def q_moe(x: torch.Tensor, router_logits: torch.Tensor, gate: tuple, up: tuple, 
     two kernels, ``w_e * silu(..) * up_e(..)``, are held with 11 significant bits.  ``x`` is ``[T, H]`` bf16 or
     fp16; ``gate``, ``up`` and ``down`` are ``(codes, scale, zero_point or None)`` with codes
     ``[E, I, H/2]``, ``[E, I, H/2]``, ``[E, H, I/2]`` in the layout of :func:`q_linear`, scale / zero_point
-    one fp16 per group of ``group_size`` (a multiple of 32).  More than 32 tokens run 32 at a time.
+    one fp16 per group of ``group_size`` (a multiple of 32).  More than 32 tokens run 32 at a time,
+    and each 32 read their experts again: for prompts of many hundreds the experts' linears one by one are
+    faster (64 experts, 8 to a token, 4096 x 1376: 512 tokens 3.0 ms here and 4.5 ms there, 2048 12 and 5.1 ms).
     An expert whose logit is ``-inf`` is not used; a token with no expert left yields zeros, one with NaN
     or ``+inf`` logits, or with NaN or infinite ``x``, yields NaN.  No reference counterpart
     (the reference runs each expert's linears)."""

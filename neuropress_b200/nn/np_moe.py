@@ -7,8 +7,11 @@ keeps its experts as separate linears; lowered one by one (:class:`NPLinear`) a 
 three kernels per chosen expert and needs the choice on the host.  :meth:`NPMoE.from_experts` stacks
 their packed weights -- same bytes, same layout, expert after expert -- and ``forward`` runs the router
 as it is and then ``kernels.q_moe``: no host synchronisation, so it can be captured in a CUDA graph.
-More than 32 tokens run 32 at a time.  Casting the module casts the router only.  The stacked weights are copies, and the block is not taken
-apart again by ``unlower_model``: keep the lowered experts where that is wanted.  No reference counterpart.
+More than 32 tokens run 32 at a time, each 32 reading their experts again: prompts of many hundreds of
+tokens are faster through the lowered experts (64 experts, 8 to a token, 4096 x 1376, 2048 tokens: 12 ms
+here, 5.1 ms there).  Casting the module casts the router only.  The stacked weights are copies, and the
+block is not taken apart again by ``unlower_model``: keep the lowered experts where that is wanted.  No
+reference counterpart.
 """
 
 from __future__ import annotations
